@@ -116,7 +116,8 @@ int sdpa_b200_dropout_mask(uint64_t seed, uint64_t offset, int64_t B, int64_t S_
 const char* sdpa_b200_strerror(int status);
 
 /* Device status word of the current device: bit 0 = a bounded wait timed out
- * inside a kernel.  Synchronises `stream`, reads the word and clears it. */
+ * inside a kernel, bit 1 = an index (page id, length, position) outside its
+ * range was met and left out.  Synchronises `stream`, reads the word and clears it. */
 int sdpa_b200_device_status(unsigned int* word, void* stream);
 
 /* Bound (nanoseconds) of every device-side wait; 0 restores the default (2 s). */
@@ -172,6 +173,78 @@ int sdpa_b200_bwd_noalloc(int dtype, const void* q, const void* k, const void* v
  *   (with n = 4 the last interval is not recorded).
  * NULL turns it off. */
 int sdpa_b200_set_bwd_events(void* const* events, int n);
+
+/* ---- Head norms with the position rotation, and the paged cache.
+ * No counterparts in the reference (its layer takes queries and keys as they
+ * are, mha.py:103-129, and serves [B, S, D] tensors).  Common rules: D and D_v
+ * are multiples of 8 up to 128; data pointers are 16-byte aligned; a token's
+ * heads are dense and `stride` elements (a multiple of 8 for fp16, 4 for
+ * float) lie between tokens; int32 arrays are device memory that only the
+ * kernels read.  Index values outside their ranges reach no memory: they raise
+ * bit 1 of the device status word (sdpa_b200_device_status).
+ *
+ * Rotation: table is float32 [max_positions, rotary_dim], cos | sin of
+ * position * base^(-2i/rotary_dim); rotary_dim a multiple of 8, 0 for none;
+ * pairs are (i, i + rotary_dim/2), or (2i, 2i+1) with interleaved != 0.
+ * Norm: x * rsqrt(mean(x^2) + eps) * weight [D] (of weight_dtype: dtype or
+ * SDPA_B200_F32); weight NULL: none.  Norm first, then rotation, in fp32,
+ * rounded once. */
+
+/* q_out, k_out [tokens, heads, D] (dense) of q and k; positions [tokens], or
+ * NULL: token index modulo `period`.  Positions outside the table are clamped
+ * to it.  Zero tokens or heads leave that side out.  Outputs must not overlap
+ * inputs. */
+int sdpa_b200_qk_norm_rope(int dtype, const void* q, int64_t q_tokens, int64_t q_heads, int64_t q_stride,
+                           const int32_t* q_positions, int64_t q_period, const void* k, int64_t k_tokens,
+                           int64_t k_heads, int64_t k_stride, const int32_t* k_positions, int64_t k_period, int64_t D,
+                           const void* q_weight, const void* k_weight, int weight_dtype, float eps, const float* table,
+                           int64_t max_positions, int64_t rotary_dim, int interleaved, void* q_out, void* k_out,
+                           void* stream);
+
+/* Its gradient: dq, dk (dense) and, for weights given, dq_weight, dk_weight
+ * (weight_dtype), summed without atomics over at most 592 blocks' partial sums
+ * in the workspace (needed only with a weight). */
+size_t sdpa_b200_qk_norm_rope_bwd_workspace_bytes(int64_t D);
+int sdpa_b200_qk_norm_rope_bwd(int dtype, const void* q, const void* dq_out, int64_t q_tokens, int64_t q_heads,
+                               int64_t q_stride, int64_t dq_out_stride, const int32_t* q_positions, int64_t q_period,
+                               const void* k, const void* dk_out, int64_t k_tokens, int64_t k_heads, int64_t k_stride,
+                               int64_t dk_out_stride, const int32_t* k_positions, int64_t k_period, int64_t D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                               const float* table, int64_t max_positions, int64_t rotary_dim, int interleaved, void* dq,
+                               void* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* The paged cache: pools k_pages [num_pages, page_size, H_kv, D] and v_pages
+ * [.., D_v], page_size a power of two from 16; sequence n's new tokens are
+ * q_start[n] .. q_start[n+1]-1 of the call (q_start [seqs+1], ascending), it
+ * holds kv_len[n] tokens with them, and its key j lies at row j % page_size of
+ * page page_table[n][j / page_size] (table_width entries a sequence; entries
+ * past a sequence's keys are not read).  Tokens behind the last sequence are
+ * left alone, in the pools and in the outputs.
+ *
+ * append writes k [tokens, H_kv, D] (normed and rotated by its position) and v
+ * [tokens, H_kv, D_v] to the pools, and q (NULL: none), normed and rotated
+ * likewise, to q_out [tokens, H_q, D]. */
+int sdpa_b200_paged_append(int dtype, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, int64_t tokens, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v,
+                           const void* q_weight, const void* k_weight, int weight_dtype, float eps, const float* table,
+                           int64_t max_positions, int64_t rotary_dim, int interleaved, void* q_out, void* k_pages,
+                           void* v_pages, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                           int64_t table_width, const int32_t* kv_len, const int32_t* q_start, int64_t seqs,
+                           void* stream);
+
+/* Attention of new tokens q [tokens, H_q, D] over their sequences' cached keys:
+ * out [tokens, H_q, D_v], stats [tokens, H_q] as in sdpa_b200_fwd.  H_q is a
+ * multiple of H_kv (query head h reads KV head h / (H_q / H_kv)).  causal != 0:
+ * a token sees the keys up to its own position; else all kv_len.  The workspace
+ * (16-byte aligned) is the caller's until the call's work has finished. */
+size_t sdpa_b200_paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs, int64_t H_q, int64_t H_kv, int64_t D,
+                                       int64_t D_v);
+int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* out,
+                         float* stats, int64_t tokens, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v,
+                         int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                         const int32_t* kv_len, const int32_t* q_start, int64_t seqs, float scale, int causal,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ABI version (major*100 + minor). */
 int sdpa_b200_version(void);

@@ -9,9 +9,11 @@ Kernels live in csrc/ and are reached through the C ABI of include/sdpa_b200.h
 """
 from .ops import (InvalidArgumentError, KernelError, device_status, dropout_mask, kernel_path, last_launch_count,
                   sdpa, sdpa_bshd, sdpa_grad, sdpa_grad_bshd)
+from .rotary import qk_norm_rope, qk_norm_rope_grad, rotary_table
+from .paged import paged_append, paged_sdpa
 from . import autograd, pipeline, sharding  # noqa: F401
 from .mha import MHA  # noqa: F401
 from ._lib import LIB_PATH  # noqa: F401
 
 __all__ = ["sdpa", "sdpa_grad", "sdpa_bshd", "sdpa_grad_bshd", "dropout_mask", "device_status", "kernel_path", "last_launch_count",
-           "InvalidArgumentError", "KernelError", "autograd", "pipeline", "sharding", "MHA"]
+           "rotary_table", "qk_norm_rope", "qk_norm_rope_grad", "paged_append", "paged_sdpa", "InvalidArgumentError", "KernelError", "autograd", "pipeline", "sharding", "MHA"]

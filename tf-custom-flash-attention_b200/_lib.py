@@ -64,6 +64,22 @@ def lib() -> ctypes.CDLL:
     L.sdpa_b200_version.restype = ci
     L.sdpa_b200_set_bwd_events.argtypes = [vp, ci]
     L.sdpa_b200_set_bwd_events.restype = ci
+    L.sdpa_b200_qk_norm_rope.argtypes = [ci, vp, i64, i64, i64, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, ci, f32,
+                                         vp, i64, i64, ci, vp, vp, vp]
+    L.sdpa_b200_qk_norm_rope.restype = ci
+    L.sdpa_b200_qk_norm_rope_bwd_workspace_bytes.argtypes = [i64]
+    L.sdpa_b200_qk_norm_rope_bwd_workspace_bytes.restype = sz
+    L.sdpa_b200_qk_norm_rope_bwd.argtypes = [ci, vp, vp, i64, i64, i64, i64, vp, i64, vp, vp, i64, i64, i64, i64, vp, i64,
+                                             i64, vp, vp, ci, f32, vp, i64, i64, ci, vp, vp, vp, vp, vp, sz, vp]
+    L.sdpa_b200_qk_norm_rope_bwd.restype = ci
+    L.sdpa_b200_paged_append.argtypes = [ci, vp, i64, vp, i64, vp, i64, i64, i64, i64, i64, i64, vp, vp, ci, f32, vp, i64,
+                                         i64, ci, vp, vp, vp, i64, i64, vp, i64, vp, vp, i64, vp]
+    L.sdpa_b200_paged_append.restype = ci
+    L.sdpa_b200_paged_workspace_bytes.argtypes = [ci, i64, i64, i64, i64, i64, i64]
+    L.sdpa_b200_paged_workspace_bytes.restype = sz
+    L.sdpa_b200_paged_sdpa.argtypes = [ci, vp, i64, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, i64, vp, vp, i64,
+                                       f32, ci, vp, sz, vp]
+    L.sdpa_b200_paged_sdpa.restype = ci
     _lib = L
     return L
 
@@ -79,4 +95,6 @@ EXPORTS = (
     "sdpa_b200_test_wait_timeout", "sdpa_b200_path", "sdpa_b200_last_launch_count", "sdpa_b200_version",
     "sdpa_b200_bwd_noalloc", "sdpa_b200_bwd_dstats", "sdpa_b200_set_bwd_events", "sdpa_b200_fwd_bshd",
     "sdpa_b200_bwd_bshd", "sdpa_b200_last_error_detail",
+    "sdpa_b200_qk_norm_rope", "sdpa_b200_qk_norm_rope_bwd_workspace_bytes", "sdpa_b200_qk_norm_rope_bwd",
+    "sdpa_b200_paged_append", "sdpa_b200_paged_workspace_bytes", "sdpa_b200_paged_sdpa",
 )

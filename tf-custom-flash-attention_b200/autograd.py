@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import ops, rotary
 
 
 class SdpaFunction(torch.autograd.Function):
@@ -72,3 +72,27 @@ def sdpa_with_stats(q, k, v, seed, offset, dropout: float = 0.0, scale: float = 
     """Differentiable attention returning (o, stats) like test.py:14-17; with
     differentiable_stats=True a loss on stats also reaches q and k."""
     return SdpaFunction.apply(q, k, v, seed, offset, dropout, scale, causal_mask, differentiable_stats)
+
+
+class QKNormRopeFunction(torch.autograd.Function):
+    """Head norms and rotation of q and k (rotary.qk_norm_rope); table and positions get no gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
+        out = rotary.qk_norm_rope(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, table, q_positions, k_positions)
+        ctx.attrs = (eps, interleaved)
+        return out
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, table, q_positions, k_positions = ctx.saved_tensors
+        grads = rotary.qk_norm_rope_grad(q, k, dq_out, dk_out, q_weight, k_weight, table, q_positions, k_positions,
+                                         *ctx.attrs)
+        return (*grads, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, table=None, q_positions=None, k_positions=None, eps: float = 1e-6,
+                 interleaved: bool = False):
+    """Differentiable ``rotary.qk_norm_rope``: gradients for q, k and the norm weights."""
+    return QKNormRopeFunction.apply(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)

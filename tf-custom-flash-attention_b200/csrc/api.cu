@@ -11,7 +11,9 @@
 #include <mutex>
 
 #include "host.cuh"
+#include "paged_mma.cuh"
 #include "ptx.cuh"
+#include "rotary.cuh"
 
 using namespace sdpa_b200;
 using namespace sdpa_b200::host;
@@ -368,7 +370,8 @@ int sdpa_b200_device_status(unsigned int* word, void* stream) {
   if (cudaMemcpyFromSymbol(&w, g_status_word, sizeof(w)) != cudaSuccess) return SDPA_B200_ECUDA;
   if (cudaMemcpyToSymbol(g_status_word, &zero, sizeof(zero)) != cudaSuccess) return SDPA_B200_ECUDA;
   if (status_exchange_fwd_tc(&w) || status_exchange_bwd_tc(&w) || status_exchange_tf32(&w) || status_exchange_simt_fwd_f16(&w) ||
-      status_exchange_simt_fwd_f32(&w) || status_exchange_simt_bwd_f16(&w) || status_exchange_simt_bwd_f32(&w)) return SDPA_B200_ECUDA;
+      status_exchange_simt_fwd_f32(&w) || status_exchange_simt_bwd_f16(&w) || status_exchange_simt_bwd_f32(&w) ||
+      status_exchange_rotary(&w) || status_exchange_paged(&w)) return SDPA_B200_ECUDA;
   if (word) *word = w;
   return (w & kStatusTimeout) ? SDPA_B200_ETIMEOUT : SDPA_B200_OK;
 }
@@ -403,6 +406,201 @@ int sdpa_b200_set_bwd_events(void* const* events, int n) {
 }
 
 int sdpa_b200_version(void) { return 100; }
+
+}  // extern "C"
+
+// ------------------------------------- head norms, rotation, the paged cache
+namespace {
+
+// Rows are read and written in 16-byte words (fp16) or eight features a lane.
+bool serving_shape(int dtype, int64_t D) {
+  return (dtype == SDPA_B200_F16 || dtype == SDPA_B200_F32) && D >= 8 && D % 8 == 0;
+}
+bool stride_ok(int dtype, int64_t stride, int64_t row) {
+  return stride >= row && stride % (dtype == SDPA_B200_F16 ? 8 : 4) == 0;
+}
+constexpr int64_t kIntMax = 0x7fffffffLL;
+
+// The norm's and rotation's arguments, shared by the three entry points.
+int fill_rotary(rotary::Params& r, int dtype, int64_t D, const void* q_weight, const void* k_weight, int weight_dtype,
+                float eps, const float* table, int64_t max_positions, int64_t rotary_dim, int interleaved) {
+  std::memset(&r, 0, sizeof(r));
+  if (!serving_shape(dtype, D)) return SDPA_B200_EINVAL;
+  if (D > 128) return SDPA_B200_EUNSUPPORTED;
+  if ((q_weight || k_weight) && weight_dtype != dtype && weight_dtype != SDPA_B200_F32) return SDPA_B200_EINVAL;
+  if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 8 != 0) return SDPA_B200_EINVAL;
+  if (rotary_dim > 0 && (!table || !aligned16(table) || max_positions < 1 || max_positions > kIntMax)) return SDPA_B200_EINVAL;
+  r.D = static_cast<int>(D);
+  r.q.weight = q_weight;
+  r.k.weight = k_weight;
+  r.weight_f32 = weight_dtype == SDPA_B200_F32 ? 1 : 0;
+  r.eps = eps;
+  r.table = rotary_dim > 0 ? table : nullptr;
+  r.max_positions = static_cast<int>(rotary_dim > 0 ? max_positions : 0);
+  r.rot = static_cast<int>(rotary_dim);
+  r.interleaved = interleaved ? 1 : 0;
+  return SDPA_B200_OK;
+}
+
+// One side of qk_norm_rope; no tokens or heads: the side is empty.
+int fill_stream(rotary::Stream& s, int dtype, int64_t D, const void* x, int64_t tokens, int64_t heads, int64_t stride,
+                const int32_t* positions, int64_t period, void* y) {
+  if (tokens < 0 || heads < 0 || tokens > kIntMax || heads > 65535) return SDPA_B200_EINVAL;
+  if (tokens == 0 || heads == 0) {
+    s.tokens = s.heads = 0;
+    s.period = 1;
+    return SDPA_B200_OK;
+  }
+  if (!x || !y || !aligned16(x) || !aligned16(y) || !stride_ok(dtype, stride, heads * D)) return SDPA_B200_EINVAL;
+  if (!positions && (period < 1 || period > kIntMax)) return SDPA_B200_EINVAL;
+  s.x = x;
+  s.y = y;
+  s.stride = stride;
+  s.positions = positions;
+  s.tokens = static_cast<int>(tokens);
+  s.heads = static_cast<int>(heads);
+  s.period = static_cast<int>(positions ? 1 : period);
+  return SDPA_B200_OK;
+}
+
+int fill_view(PagedView& v, const int32_t* page_table, int64_t table_width, const int32_t* kv_len, const int32_t* q_start,
+              int64_t seqs, int64_t num_pages, int64_t page_size, int64_t tokens) {
+  if (seqs < 0 || tokens < 0 || table_width < 0 || num_pages < 0) return SDPA_B200_EINVAL;
+  if (seqs >= kIntMax || tokens > kIntMax || table_width > kIntMax || num_pages > kIntMax) return SDPA_B200_EINVAL;
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1))) return SDPA_B200_EINVAL;
+  if (table_width * page_size > kIntMax - 65536) return SDPA_B200_EINVAL;
+  if (seqs > 0 && (!kv_len || !q_start || (table_width > 0 && !page_table))) return SDPA_B200_EINVAL;
+  v.page_table = page_table;
+  v.kv_len = kv_len;
+  v.q_start = q_start;
+  v.seqs = static_cast<int>(seqs);
+  v.width = static_cast<int>(table_width);
+  v.num_pages = static_cast<int>(num_pages);
+  v.tokens = static_cast<int>(tokens);
+  v.page_shift = 0;
+  while ((int64_t(1) << v.page_shift) < page_size) ++v.page_shift;
+  return SDPA_B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sdpa_b200_qk_norm_rope(int dtype, const void* q, int64_t q_tokens, int64_t q_heads, int64_t q_stride,
+                           const int32_t* q_positions, int64_t q_period, const void* k, int64_t k_tokens, int64_t k_heads,
+                           int64_t k_stride, const int32_t* k_positions, int64_t k_period, int64_t D, const void* q_weight,
+                           const void* k_weight, int weight_dtype, float eps, const float* table, int64_t max_positions,
+                           int64_t rotary_dim, int interleaved, void* q_out, void* k_out, void* stream) {
+  t_launches = 0;
+  rotary::Params r;
+  if (int e = fill_rotary(r, dtype, D, q_weight, k_weight, weight_dtype, eps, table, max_positions, rotary_dim, interleaved))
+    return e;
+  if (int e = fill_stream(r.q, dtype, D, q, q_tokens, q_heads, q_stride, q_positions, q_period, q_out)) return e;
+  if (int e = fill_stream(r.k, dtype, D, k, k_tokens, k_heads, k_stride, k_positions, k_period, k_out)) return e;
+  if (!r.q.tokens && !r.k.tokens) return SDPA_B200_OK;
+  return launch_rotary_fwd(dtype, r, static_cast<cudaStream_t>(stream), &t_launches);
+}
+
+size_t sdpa_b200_qk_norm_rope_bwd_workspace_bytes(int64_t D) {
+  return D < 1 ? 0 : static_cast<size_t>(rotary::kGradBlocks) * 2 * static_cast<size_t>(D) * sizeof(float);
+}
+
+int sdpa_b200_qk_norm_rope_bwd(int dtype, const void* q, const void* dq_out, int64_t q_tokens, int64_t q_heads,
+                               int64_t q_stride, int64_t dq_out_stride, const int32_t* q_positions, int64_t q_period,
+                               const void* k, const void* dk_out, int64_t k_tokens, int64_t k_heads, int64_t k_stride,
+                               int64_t dk_out_stride, const int32_t* k_positions, int64_t k_period, int64_t D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, float eps, const float* table,
+                               int64_t max_positions, int64_t rotary_dim, int interleaved, void* dq, void* dk,
+                               void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  t_launches = 0;
+  rotary::Params r;
+  if (int e = fill_rotary(r, dtype, D, q_weight, k_weight, weight_dtype, eps, table, max_positions, rotary_dim, interleaved))
+    return e;
+  if (int e = fill_stream(r.q, dtype, D, q, q_tokens, q_heads, q_stride, q_positions, q_period, dq)) return e;
+  if (int e = fill_stream(r.k, dtype, D, k, k_tokens, k_heads, k_stride, k_positions, k_period, dk)) return e;
+  if (r.q.tokens && (!dq_out || !aligned16(dq_out) || !stride_ok(dtype, dq_out_stride, q_heads * D))) return SDPA_B200_EINVAL;
+  if (r.k.tokens && (!dk_out || !aligned16(dk_out) || !stride_ok(dtype, dk_out_stride, k_heads * D))) return SDPA_B200_EINVAL;
+  if ((!q_weight) != (!dq_weight) || (!k_weight) != (!dk_weight)) return SDPA_B200_EINVAL;
+  if (q_weight || k_weight) {
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3u) ||
+        workspace_bytes < sdpa_b200_qk_norm_rope_bwd_workspace_bytes(D))
+      return SDPA_B200_EWORKSPACE;
+  }
+  r.q.dy = dq_out;
+  r.q.dy_stride = dq_out_stride;
+  r.k.dy = dk_out;
+  r.k.dy_stride = dk_out_stride;
+  r.dw_q = dq_weight;
+  r.dw_k = dk_weight;
+  r.partial = static_cast<float*>(workspace);
+  return launch_rotary_bwd(dtype, r, static_cast<cudaStream_t>(stream), &t_launches);
+}
+
+int sdpa_b200_paged_append(int dtype, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, int64_t tokens, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v,
+                           const void* q_weight, const void* k_weight, int weight_dtype, float eps, const float* table,
+                           int64_t max_positions, int64_t rotary_dim, int interleaved, void* q_out, void* k_pages,
+                           void* v_pages, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                           int64_t table_width, const int32_t* kv_len, const int32_t* q_start, int64_t seqs, void* stream) {
+  t_launches = 0;
+  rotary::Params r;
+  if (int e = fill_rotary(r, dtype, D, q_weight, k_weight, weight_dtype, eps, table, max_positions, rotary_dim, interleaved))
+    return e;
+  if (!serving_shape(dtype, D_v) || H_kv < 1) return SDPA_B200_EINVAL;
+  if (D_v > 128) return SDPA_B200_EUNSUPPORTED;
+  if (int e = fill_view(r.view, page_table, table_width, kv_len, q_start, seqs, num_pages, page_size, tokens)) return e;
+  if (tokens == 0 || seqs == 0) return SDPA_B200_OK;
+  if (int e = fill_stream(r.q, dtype, D, q, q ? tokens : 0, H_q, q_stride, nullptr, 1, q_out)) return e;
+  if (int e = fill_stream(r.k, dtype, D, k, tokens, H_kv, k_stride, nullptr, 1, k_pages)) return e;
+  if (int e = fill_stream(r.v, dtype, D_v, v, tokens, H_kv, v_stride, nullptr, 1, v_pages)) return e;
+  r.k.y = nullptr;  // keys go to their pages
+  r.v.y = nullptr;
+  r.D_v = static_cast<int>(D_v);
+  r.k_pages = k_pages;
+  r.v_pages = v_pages;
+  return launch_paged_append(dtype, r, static_cast<cudaStream_t>(stream), &t_launches);
+}
+
+size_t sdpa_b200_paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs, int64_t H_q, int64_t H_kv, int64_t D,
+                                       int64_t D_v) {
+  if (tokens < 1 || seqs < 1 || H_q < 1 || H_kv < 1 || D < 1 || D_v < 1) return 0;
+  return paged_workspace_bytes(dtype, tokens, seqs, H_q, H_kv, D, D_v);
+}
+
+int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* out,
+                         float* stats, int64_t tokens, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v,
+                         int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                         const int32_t* kv_len, const int32_t* q_start, int64_t seqs, float scale, int causal,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  t_launches = 0;
+  if (!serving_shape(dtype, D) || !serving_shape(dtype, D_v)) return SDPA_B200_EINVAL;
+  if (D > 128 || D_v > 128) return SDPA_B200_EUNSUPPORTED;
+  if (H_kv < 1 || H_q < H_kv || H_q % H_kv != 0) return SDPA_B200_EINVAL;
+  paged::Params p;
+  std::memset(&p, 0, sizeof(p));
+  if (int e = fill_view(p.view, page_table, table_width, kv_len, q_start, seqs, num_pages, page_size, tokens)) return e;
+  if (tokens == 0 || seqs == 0) return SDPA_B200_OK;
+  if (H_q > kIntMax / tokens) return SDPA_B200_EINVAL;  // packed rows are counted in 32 bits
+  if (!q || !out || !stats || !aligned16(q) || !aligned16(out) || !stride_ok(dtype, q_stride, H_q * D)) return SDPA_B200_EINVAL;
+  if (num_pages > 0 && (!k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages))) return SDPA_B200_EINVAL;
+  if (!workspace || !aligned16(workspace) ||
+      workspace_bytes < sdpa_b200_paged_workspace_bytes(dtype, tokens, seqs, H_q, H_kv, D, D_v))
+    return SDPA_B200_EWORKSPACE;
+  p.q = q;
+  p.q_stride = q_stride;
+  p.k_pages = k_pages;
+  p.v_pages = v_pages;
+  p.out = out;
+  p.stats = stats;
+  p.H_q = static_cast<int>(H_q);
+  p.H_kv = static_cast<int>(H_kv);
+  p.G = static_cast<int>(H_q / H_kv);
+  p.D = static_cast<int>(D);
+  p.D_v = static_cast<int>(D_v);
+  p.scale_log2 = scale * kLog2e;
+  p.causal = causal ? 1 : 0;
+  return launch_paged_sdpa(dtype, p, workspace, static_cast<cudaStream_t>(stream), &t_launches);
+}
 
 }  // extern "C"
 

@@ -1,0 +1,163 @@
+"""Serving: the paged key/value cache, its write and the attention that reads it.
+
+The cache is two pools, ``k_pages`` [pages, page_size, H_kv, D] and ``v_pages``
+[pages, page_size, H_kv, D_v].  A call takes the new tokens of several
+sequences one behind the other, [T, H, D], with three int32 device tensors:
+
+    q_start    [N+1]   sequence n's new tokens are q_start[n] .. q_start[n+1]-1
+    kv_len     [N]     tokens it has cached once its new ones are written
+    page_table [N, M]  its key j lies at row j % page_size of page_table[n, j // page_size]
+
+so new token i of sequence n is at position kv_len[n] - (q_start[n+1] -
+q_start[n]) + i.  The kernels read these on the device, the host never does: a
+captured graph replays with whatever they hold then.  Rows behind the last
+sequence (T past q_start[N], the padding of a captured batch) are neither
+written to the cache nor to the outputs.  A page id outside the pool reads as
+zeros and is not written, a length past the table's capacity is clamped to it,
+and both raise bit 1 of ``device_status``.
+
+``paged_append`` writes new keys and values, with the head norms and the
+position rotation of ``rotary.qk_norm_rope`` applied on the way (and to the
+queries, in the same launch); ``paged_sdpa`` attends.  No counterparts in the
+reference, which serves [B, S, D] tensors only.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops import InvalidArgumentError, _check
+from .rotary import _check_features, _dtype_of, _ptr, _rows, _same, _table, _weights
+
+
+def _check_batch(page_table, kv_len, q_start, ref: torch.Tensor):
+    for x, name, dim in ((page_table, "page_table", 2), (kv_len, "kv_len", 1), (q_start, "q_start", 1)):
+        if x.dtype != torch.int32 or x.dim() != dim or not x.is_contiguous():
+            raise InvalidArgumentError(f"{name} must be a contiguous int32 tensor of rank {dim}")
+        _same(x, ref, name)
+    N = kv_len.shape[0]
+    if page_table.shape[0] != N or q_start.shape[0] != N + 1:
+        raise InvalidArgumentError("page_table must be [N, M], kv_len [N] and q_start [N+1]")
+    return N
+
+
+def _check_pools(k_pages, v_pages, ref: torch.Tensor):
+    for x, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if x.dim() != 4 or not x.is_contiguous():
+            raise InvalidArgumentError(f"{name} must be a contiguous [pages, page_size, H_kv, D] tensor")
+        if x.dtype != ref.dtype:
+            raise InvalidArgumentError("all floating-point inputs must share dtype T")
+        _same(x, ref, name)
+        if x.data_ptr() % 16:
+            raise InvalidArgumentError(f"{name} must start at a multiple of 16 bytes")
+    if k_pages.shape[:3] != v_pages.shape[:3]:
+        raise InvalidArgumentError("k_pages and v_pages must have the same pages, page size and heads")
+    P, page, H_kv, D = k_pages.shape
+    if page < 16 or page > 65536 or page & (page - 1):
+        raise InvalidArgumentError(f"page_size must be a power of two from 16 to 65536, got {page}")
+    _check_features(D)
+    _check_features(v_pages.shape[3], "value feature size")
+    return P, page, H_kv, D, v_pages.shape[3]
+
+
+def _check_tokens(x: torch.Tensor, name: str, T: int, D: int, H, dtype):
+    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D or (H is not None and x.shape[1] != H):
+        raise InvalidArgumentError(f"{name} must be [{T}, {'H' if H is None else H}, {D}], got {list(x.shape)}")
+    if x.dtype != dtype:
+        raise InvalidArgumentError("all floating-point inputs must share dtype T")
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 kv_len: torch.Tensor, q_start: torch.Tensor, q=None, q_weight=None, k_weight=None, table=None,
+                 eps: float = 1e-6, interleaved: bool = False):
+    """Writes k [T, H_kv, D] and v [T, H_kv, D_v] at their positions in the pools.
+
+    With ``k_weight`` the keys are normed, with ``table`` (``rotary_table``)
+    rotated by their position, before they are written; ``q`` [T, H_q, D] gets
+    the same (with ``q_weight``) and is returned, else None.  Rows of the result
+    behind the last sequence are not written.  Positions that two sequences
+    share (a page entered in both tables) must get the same rows from both."""
+    dt = _dtype_of(k)
+    if k.dim() != 3:
+        raise InvalidArgumentError(f"k must be [T, H_kv, D] but is rank {k.dim()}")
+    _same(k, k, "k")
+    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, k)
+    N = _check_batch(page_table, kv_len, q_start, k)
+    T = k.shape[0]
+    _check_tokens(k, "k", T, D, H_kv, k.dtype)
+    _check_tokens(v, "v", T, D_v, H_kv, k.dtype)
+    _same(v, k, "v")
+    if q is not None:
+        _check_tokens(q, "q", T, D, None, k.dtype)
+        _same(q, k, "q")
+    elif q_weight is not None:
+        raise InvalidArgumentError("q_weight without q")
+    qw, kw, wdt = _weights(q_weight, k_weight, k, D)
+    table, max_pos, rot = _table(table, k, D)
+    align = 8 if dt == _lib.F16 else 4
+    kx, ks = _rows(k, align)
+    vx, vs = _rows(v, align)
+    q_out, qx, qs, H_q = None, None, 0, 0
+    if q is not None:
+        qx, qs = _rows(q, align)
+        H_q = q.shape[1]
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    with torch.cuda.device(k.device):
+        st = torch.cuda.current_stream().cuda_stream
+        rc = _lib.lib().sdpa_b200_paged_append(
+            dt, _ptr(qx), qs, kx.data_ptr(), ks, vx.data_ptr(), vs, T, H_q, H_kv, D, D_v, _ptr(qw), _ptr(kw), wdt,
+            float(eps), _ptr(table), max_pos, rot, int(bool(interleaved)), _ptr(q_out), k_pages.data_ptr(),
+            v_pages.data_ptr(), P, page, page_table.data_ptr(), page_table.shape[1], kv_len.data_ptr(),
+            q_start.data_ptr(), N, st)
+    _check(rc)
+    return q_out
+
+
+def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+               kv_len: torch.Tensor, q_start: torch.Tensor, scale: float = 1.0, causal_mask: bool = True, *, out=None):
+    """Attention of new tokens q [T, H_q, D] over the cached keys of their sequences.
+
+    Returns (output [T, H_q, D_v] T, stats [T, H_q] float32), stats as in
+    ``sdpa``: max + ln(sum + 1e-6) of the scaled scores.  H_q is a multiple of
+    H_kv; query head h reads KV head h // (H_q / H_kv).  With ``causal_mask`` a
+    token sees the keys up to its own position, else all kv_len of its sequence;
+    one that sees none gets zeros and stats of -1e9.  ``out`` may pass
+    (output, stats) to write into; rows behind the last sequence keep what they
+    held (and hold anything in a result allocated here).  A NaN or infinity
+    cached behind a sequence's kv_len reaches nothing; one at a position that
+    only later tokens of the same chunk see may reach the chunk's earlier rows."""
+    dt = _dtype_of(q)
+    if q.dim() != 3:
+        raise InvalidArgumentError(f"q must be [T, H_q, D] but is rank {q.dim()}")
+    _same(q, q, "q")
+    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, q)
+    N = _check_batch(page_table, kv_len, q_start, q)
+    T, H_q = q.shape[0], q.shape[1]
+    _check_tokens(q, "q", T, D, None, q.dtype)
+    if H_kv < 1 or H_q < 1 or H_q % H_kv:
+        raise InvalidArgumentError("H_q must be a multiple of H_kv")
+    if out is None:
+        o = torch.empty((T, H_q, D_v), dtype=q.dtype, device=q.device)
+        stats = torch.empty((T, H_q), dtype=torch.float32, device=q.device)
+    else:
+        o, stats = out
+        if tuple(o.shape) != (T, H_q, D_v) or o.dtype != q.dtype or not o.is_contiguous():
+            raise InvalidArgumentError("out[0] must be a contiguous [T, H_q, D_v] tensor of dtype T")
+        if tuple(stats.shape) != (T, H_q) or stats.dtype != torch.float32 or not stats.is_contiguous():
+            raise InvalidArgumentError("out[1] must be a contiguous float32 [T, H_q] tensor")
+        _same(o, q, "out[0]")
+        _same(stats, q, "out[1]")
+    if T == 0 or N == 0:
+        return o, stats
+    qx, qs = _rows(q, 8 if dt == _lib.F16 else 4)
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        ws_bytes = L.sdpa_b200_paged_workspace_bytes(dt, T, N, H_q, H_kv, D, D_v)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        st = torch.cuda.current_stream().cuda_stream
+        rc = L.sdpa_b200_paged_sdpa(
+            dt, qx.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(), stats.data_ptr(), T, H_q, H_kv, D,
+            D_v, P, page, page_table.data_ptr(), page_table.shape[1], kv_len.data_ptr(), q_start.data_ptr(), N,
+            float(scale), int(bool(causal_mask)), ws.data_ptr(), ws_bytes, st)
+    _check(rc)
+    return o, stats
