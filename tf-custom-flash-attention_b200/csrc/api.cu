@@ -371,7 +371,8 @@ int sdpa_b200_device_status(unsigned int* word, void* stream) {
   if (cudaMemcpyToSymbol(g_status_word, &zero, sizeof(zero)) != cudaSuccess) return SDPA_B200_ECUDA;
   if (status_exchange_fwd_tc(&w) || status_exchange_bwd_tc(&w) || status_exchange_tf32(&w) || status_exchange_simt_fwd_f16(&w) ||
       status_exchange_simt_fwd_f32(&w) || status_exchange_simt_bwd_f16(&w) || status_exchange_simt_bwd_f32(&w) ||
-      status_exchange_rotary(&w) || status_exchange_paged(&w)) return SDPA_B200_ECUDA;
+      status_exchange_rotary(&w) || status_exchange_paged(&w) ||
+      status_exchange_paged_tc(&w)) return SDPA_B200_ECUDA;
   if (word) *word = w;
   return (w & kStatusTimeout) ? SDPA_B200_ETIMEOUT : SDPA_B200_OK;
 }
@@ -599,6 +600,8 @@ int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void*
   p.D_v = static_cast<int>(D_v);
   p.scale_log2 = scale * kLog2e;
   p.causal = causal ? 1 : 0;
+  p.timeout_ns = g_timeout_ns.load();
+  if (int r = bind_context()) return r;
   return launch_paged_sdpa(dtype, p, workspace, static_cast<cudaStream_t>(stream), &t_launches);
 }
 

@@ -1,4 +1,5 @@
-// Translation unit: attention over the paged cache
+// Translation unit: attention over the paged cache, the kernels for few rows
+// and the choice between them and paged_tc.cu's for chunks
 #include "host.cuh"
 #include "paged_mma.cuh"
 
@@ -73,16 +74,24 @@ int launch_mma(const paged::Params& p, void* ws, int mt, cudaStream_t st, int* l
 
 }  // namespace
 
+// Chunks go to the tcgen05 kernel: fp16, a head group that fits its 128-row
+// tiles, and more than one 16-row tile of packed rows a sequence on average
+// (the lengths themselves are on the device).
+static bool use_tc(int dtype, int64_t tokens, int64_t seqs, int64_t group) {
+  return dtype == SDPA_B200_F16 && group <= 128 && tokens * group > 16 * seqs;
+}
+
 size_t sdpa_b200::paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs, int64_t H_q, int64_t H_kv, int64_t D,
                                         int64_t D_v) {
-  (void)dtype;
+  if (use_tc(dtype, tokens, seqs, H_q / H_kv)) return paged_tc_workspace_bytes(static_cast<int>(D_v));
   const int mt = row_tiles_of(tokens, seqs, H_q / H_kv);
   return layout_of(max_ctas(), paged::kRows * mt, bucket_of(static_cast<int>(D), static_cast<int>(D_v))).bytes;
 }
 
 int sdpa_b200::launch_paged_sdpa(int dtype, paged::Params p, void* workspace, cudaStream_t st, int* launches) {
   const int mt = row_tiles_of(p.view.tokens, p.view.seqs, p.G);
-  p.max_rows = 0x7fffffff;
+  p.sms = num_sms();
+  if (use_tc(dtype, p.view.tokens, p.view.seqs, p.G)) return launch_paged_tc(p, workspace, st, launches);
   const bool small = bucket_of(p.D, p.D_v) == 64;
   if (dtype == SDPA_B200_F16)
     return small ? launch_mma<__half, 64>(p, workspace, mt, st, launches) : launch_mma<__half, 128>(p, workspace, mt, st, launches);

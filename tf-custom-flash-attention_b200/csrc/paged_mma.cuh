@@ -49,11 +49,12 @@ struct Params {
   int H_q, H_kv, G, D, D_v;
   float scale_log2;
   int causal;
-  int max_rows;           // sequences with more packed rows are another kernel's
   // workspace
   float* part_o;          // [ctas, 2, rows, DB] unnormalised sums
   float2* part_ml;        // [ctas, 2, rows] (max, sum), log2 units
   int4* part_item;        // [ctas] (sequence, head, row tile, CTAs after this one that hold the rest; -1: none)
+  int sms;                // SMs of the device
+  uint64_t timeout_ns;
 };
 
 __device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -103,8 +104,7 @@ __device__ __forceinline__ uint4 ldg16(const void* p) {
 }
 
 __device__ __forceinline__ int row_tiles(const Params& p, const SeqLens& s, int rows) {
-  const int64_t r = static_cast<int64_t>(s.count) * p.G;
-  return r > p.max_rows ? 0 : static_cast<int>((r + rows - 1) / rows);
+  return static_cast<int>((static_cast<int64_t>(s.count) * p.G + rows - 1) / rows);
 }
 __device__ __forceinline__ int key_tiles(const SeqLens& s) { return s.held > 0 ? (s.held + kTile - 1) / kTile : 1; }
 // Tiles of all items of sequence n.
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
     const int tiles = static_cast<int>(min(static_cast<int64_t>(nt - tile0), w1 - w));
 
     // ---- rows of this warp
-    const int total_rows = sl.count * p.G;  // <= max_rows or the grid's own bound
+    const int total_rows = sl.count * p.G;
     const int r0 = (rtile * MT + mt) * kRows;
     const int ra = r0 + g, rb = r0 + g + 8;
     const bool va = ra < total_rows, vb = rb < total_rows;

@@ -1,0 +1,581 @@
+// Attention of chunks of new tokens over the paged cache on the 5th-generation
+// tensor cores, fp16 in, fp32 accumulate.
+//
+// Bound: the two products (2 seen keys (D + D_v) operations a row).  The pipe
+// is the paired forward's (fwd_tc.cuh): one CTA = two 128-row tiles that share
+// every K/V tile, two softmax warpgroups alternating on the tensor pipe, one
+// TMA warp, one MMA warp.  What differs:
+//   - rows are packed (token, head of the group): a tile is floor(128 / G)
+//     tokens x G heads, so the G heads of a KV head share one reading of it;
+//     Q comes as one box (64 columns, G heads, 1 KV head, tokens) a tile;
+//   - a K/V tile of 128 keys is 128 / min(page, 128) boxes, one page each, one
+//     issued by each lane of the TMA warp (a page's boxes need its table entry
+//     first; the entries of the next tile are read a tile ahead);
+//   - keys behind the sequence are masked, and their V rows set to zero in
+//     shared memory before the product (0 * NaN is NaN);
+//   - long sequences with few rows are cut along the keys (below).
+//
+// Work: an item is a pair of row tiles of one (sequence, KV head).  With at
+// least as many items as SMs they run whole, but for the last items % SMs,
+// which are cut into floor(SMs / rest) pieces each so that the last wave is
+// full too.  With fewer, each is cut in proportion to its sequence's length, to
+// about one piece an SM.  Pieces leave unnormalised sums that merge_kernel
+// joins.  Every CTA works the cut out itself from the lengths on the device.
+#pragma once
+#include "fwd_tc.cuh"
+#include "paged_mma.cuh"
+
+namespace sdpa_b200 {
+namespace paged_tc {
+
+using paged::Params;
+using tc::kBM;
+using tc::kBN;
+using tc::warp_wait;
+
+constexpr int kThreads = 320;
+constexpr int kMergeThreads = 256;
+
+template <int DQK, int DV>
+struct Cfg {
+  static constexpr int kStages = (DQK + DV > 128) ? 2 : 4;
+  static constexpr uint32_t kQBytes = kBM * DQK * 2;  // one tile
+  static constexpr uint32_t kKBytes = kBN * DQK * 2;
+  static constexpr uint32_t kVBytes = kBN * DV * 2;
+  static constexpr uint32_t kKOff = 2 * kQBytes;
+  static constexpr uint32_t kVOff = kKOff + kStages * kKBytes;
+  static constexpr uint32_t kBarOff = kVOff + kStages * kVBytes;
+  static constexpr uint32_t kSmemBytes = kBarOff + 256 + 1024;
+  static constexpr uint32_t kTmemCols = 512;
+  static_assert(256 + 2 * DV <= 512, "TMEM budget");
+};
+
+struct Barriers {
+  uint64_t q_full;
+  uint64_t k_full[4];
+  uint64_t v_full[4];
+  uint64_t kv_empty[4];
+  uint64_t s_full[2];  // per row tile
+  uint64_t p_full[2];
+  uint64_t o_done[2];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 256, "barrier space");
+
+// ---------------------------------------------------------------- the cut
+struct Piece {
+  int seq, head, pair;  // item
+  int piece, pieces;    // its share of the item's keys
+  int slot;             // workspace slot (pieces > 1)
+};
+
+template <int THREADS>
+struct SchedSmem {
+  int64_t a[THREADS / 32], b[THREADS / 32];
+  Piece found;
+  int live;
+};
+
+// Inclusive prefix sum of x over the block, and its total.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* warp_sums, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t v = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += up;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + v;
+}
+
+__device__ __forceinline__ int pairs_of(const SeqLens& s, int tokens2) { return (s.count + tokens2 - 1) / tokens2; }
+__device__ __forceinline__ int tiles_of(const SeqLens& s) { return max(1, (s.held + kBN - 1) / kBN); }
+
+// The piece that CTA `idx` computes (from_slot: the piece in workspace slot
+// `idx`), the same for every thread; false if there is none.
+template <int THREADS>
+__device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, bool from_slot, SchedSmem<THREADS>& sm,
+                                           Piece& out) {
+  const int tokens2 = 2 * (kBM / p.G);
+  const int per = (p.view.seqs + THREADS - 1) / THREADS, n0 = threadIdx.x * per;
+  const int n1 = min(p.view.seqs, n0 + per);
+  int64_t items = 0, work = 0;
+  for (int n = n0; n < n1; ++n) {
+    const SeqLens s = seq_lens(p.view, n);
+    const int64_t pr = pairs_of(s, tokens2);
+    items += pr;
+    work += pr * tiles_of(s);
+  }
+  if (threadIdx.x == 0) sm.live = 0;
+  int64_t all_items, all_work;
+  const int64_t incl = block_scan<THREADS>(items, sm.a, all_items);
+  block_scan<THREADS>(work, sm.b, all_work);
+  all_items *= p.H_kv;
+  all_work *= p.H_kv;
+  const int64_t sms = p.sms;
+  const bool whole = all_items >= sms;  // the first `full` items run whole
+  const int64_t rest = all_items % sms, full = whole ? all_items - rest : 0;
+  const int64_t quantum = max(static_cast<int64_t>(1), (all_work + sms - 1) / sms);
+  if (from_slot) idx += full;
+  int64_t target = idx, at = (incl - items) * p.H_kv;  // first item (piece) of this thread's sequences
+  int cut = 1, piece = 0;
+  if (whole) {
+    if (idx >= full) {
+      cut = static_cast<int>(rest ? sms / rest : 1);
+      target = full + (idx - full) / cut;
+      piece = static_cast<int>((idx - full) % cut);
+    }
+  } else {
+    int64_t mine = 0, total;
+    for (int n = n0; n < n1; ++n) {
+      const SeqLens s = seq_lens(p.view, n);
+      mine += static_cast<int64_t>(pairs_of(s, tokens2)) * max(static_cast<int64_t>(1), tiles_of(s) / quantum);
+    }
+    at = (block_scan<THREADS>(mine, sm.a, total) - mine) * p.H_kv;
+  }
+  for (int n = n0; n < n1; ++n) {
+    const SeqLens s = seq_lens(p.view, n);
+    const int64_t pr = pairs_of(s, tokens2);
+    if (!whole) cut = static_cast<int>(max(static_cast<int64_t>(1), tiles_of(s) / quantum));
+    const int64_t count = pr * p.H_kv * (whole ? 1 : cut);
+    if (target >= at && target < at + count) {
+      int64_t local = target - at;
+      if (!whole) {
+        piece = static_cast<int>(local % cut);
+        local /= cut;
+      }
+      Piece f;
+      f.seq = n;
+      f.head = static_cast<int>(local / pr);
+      f.pair = static_cast<int>(pr - 1 - local % pr);  // longest causal rows first
+      f.piece = piece;
+      f.pieces = cut;
+      f.slot = static_cast<int>(idx - full);
+      sm.found = f;
+      sm.live = 1;
+    }
+    at += count;
+  }
+  __syncthreads();
+  out = sm.found;
+  return sm.live != 0;
+}
+
+// Keys [0, lim) that token i (of the sequence's new ones) sees.
+__device__ __forceinline__ int limit_of(const Params& p, const SeqLens& s, int i) {
+  return p.causal ? max(0, min(s.held, s.held - s.count + i + 1)) : s.held;
+}
+
+// Key tiles of the item's pair of row tiles, and of this piece: [j0, j1).
+struct Range {
+  int tok0;      // first token of the pair (of the sequence's new ones)
+  int n_item;    // key tiles the pair needs
+  int j0, j1;
+};
+__device__ __forceinline__ Range range_of(const Params& p, const SeqLens& s, const Piece& w) {
+  const int tokens2 = 2 * (kBM / p.G);
+  Range r;
+  r.tok0 = w.pair * tokens2;
+  const int last = min(s.count, r.tok0 + tokens2) - 1;
+  r.n_item = (limit_of(p, s, last) + kBN - 1) / kBN;
+  r.j0 = static_cast<int>(static_cast<int64_t>(r.n_item) * w.piece / w.pieces);
+  r.j1 = static_cast<int>(static_cast<int64_t>(r.n_item) * (w.piece + 1) / w.pieces);
+  return r;
+}
+
+template <int DQK, int DV>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  using C = Cfg<DQK, DV>;
+  constexpr int ST = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = tc::align1024(smem_raw);
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
+  __shared__ SchedSmem<kThreads> sched;
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], kBM);
+      mbar_init(&bars->o_done[s], 1);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  pdl_launch_dependents();
+  pdl_wait();  // before any global access and before the wait deadline starts
+  Piece w;
+  if (!find_piece<kThreads>(p, blockIdx.x, false, sched, w)) return;  // no TMEM held yet
+  if (warp == 9) tmem_alloc(&bars->tmem_base, C::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  WaitCtl ctl;
+  ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;
+  ctl.abort_flag = &bars->abort_flag;
+
+  const SeqLens sl = seq_lens(p.view, w.seq);
+  const Range rg = range_of(p, sl, w);
+  const int tpt = kBM / p.G;  // tokens of a row tile
+  const int n_kv = rg.j1 - rg.j0;
+  // key tiles per row tile within the piece; the second tile may have no tokens
+  int n_t[2];
+  {
+    const int last_a = min(sl.count, rg.tok0 + tpt) - 1;
+    n_t[0] = max(0, min(n_kv, (limit_of(p, sl, last_a) + kBN - 1) / kBN - rg.j0));
+    n_t[1] = rg.tok0 + tpt < sl.count ? n_kv : 0;
+  }
+
+  if (warp == 8) {
+    // ------------------------------------------------------ TMA producer
+    if (n_kv > 0) {
+      const int box = min(kBN, 1 << p.view.page_shift);
+      const int subs = kBN / box;                         // boxes of a column block
+      constexpr int KC = DQK / 64, VC = DV / 64;
+      const int loads = subs * (KC + VC);                 // a tile's, at most 8 * 4 = 32
+      const int sub = lane % subs, chunk = lane / subs;   // this lane's
+      const bool mine = lane < loads, is_k = chunk < KC;
+      const int page_mask = (1 << p.view.page_shift) - 1;
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        // boxes of tpt tokens x G heads: tpt * G rows of each tile
+        mbar_expect_tx(&bars->q_full, 2u * static_cast<uint32_t>(KC * tpt * p.G * 128));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+            tma_load_4d(smem + t * C::kQBytes + c * kBM * 128, &tm_q, c * 64, 0, w.head, sl.begin + rg.tok0 + t * tpt,
+                        &bars->q_full);
+      }
+      auto page_at = [&](int j) {
+        const int key = (rg.j0 + j) * kBN + sub * box;
+        return mine && j < n_kv && key < sl.held ? page_of(p.view, w.seq, key >> p.view.page_shift) : -2;
+      };
+      int page = page_at(0), issued = 0;
+      for (int j = 0; j < n_kv; ++j) {
+        const int s = j % ST;
+        const int next = page_at(j + 1);
+        if (!warp_wait(&bars->kv_empty[s], ((j / ST) & 1) ^ 1, ctl)) break;
+        const int key0 = (rg.j0 + j) * kBN;
+        const int boxes = min(subs, (sl.held - key0 + box - 1) / box);  // boxes that hold keys of the sequence
+        if (lane == 0) {
+          mbar_expect_tx(&bars->k_full[s], static_cast<uint32_t>(KC * boxes * box * 128));
+          mbar_expect_tx(&bars->v_full[s], static_cast<uint32_t>(VC * boxes * box * 128));
+        }
+        __syncwarp();
+        if (mine && sub < boxes) {  // a page id outside the pool (-1) reads as zeros
+          const int row = (key0 + sub * box) & page_mask;
+          if (is_k)
+            tma_load_4d(smem + C::kKOff + s * C::kKBytes + chunk * kBN * 128 + sub * box * 128, &tm_k, chunk * 64, w.head,
+                        row, page, &bars->k_full[s]);
+          else
+            tma_load_4d(smem + C::kVOff + s * C::kVBytes + (chunk - KC) * kBN * 128 + sub * box * 128, &tm_v,
+                        (chunk - KC) * 64, w.head, row, page, &bars->v_full[s]);
+        }
+        issued = j + 1;
+        page = next;
+      }
+      __syncwarp();
+      if (*ctl.abort_flag && lane == 0) {  // let copies in flight land before the CTA exits
+        WaitCtl drain = ctl;
+        drain.deadline_ns = globaltimer_ns() + p.timeout_ns;
+        int dummy = 0;
+        drain.abort_flag = &dummy;
+        mbar_wait(&bars->q_full, 0, drain);
+        for (int j = (issued > ST ? issued - ST : 0); j < issued; ++j) {
+          mbar_wait(&bars->k_full[j % ST], (j / ST) & 1, drain);
+          mbar_wait(&bars->v_full[j % ST], (j / ST) & 1, drain);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------- MMA issuer
+    if (lane == 0 && n_kv > 0) {
+      constexpr uint32_t idesc_qk = make_idesc(kBM, kBN, false, false, false);
+      constexpr uint32_t idesc_pv = make_idesc(kBM, DV, false, true, false);
+      const uint32_t sQ = smem_u32(smem);
+      const uint32_t sK0 = smem_u32(smem + C::kKOff);
+      const uint32_t sV0 = smem_u32(smem + C::kVOff);
+      auto issue_s = [&](int t, int j) -> bool {  // S_t = Q_t K_j^T
+        const int s = j % ST;
+        if (!mbar_wait(&bars->k_full[s], (j / ST) & 1, ctl)) return false;
+        tc_fence_after();
+        const uint32_t kbase = sK0 + s * C::kKBytes, qbase = sQ + t * C::kQBytes;
+#pragma unroll
+        for (int kk = 0; kk < DQK / 16; ++kk) {
+          const uint32_t koff = (kk >> 2) * (kBM * 128) + (kk & 3) * 32;
+          mma_f16_ss(tmem + t * 128, make_sw128_desc(qbase + koff, 16, 1024), make_sw128_desc(kbase + koff, 16, 1024),
+                     idesc_qk, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&bars->s_full[t]);
+        return true;
+      };
+      auto issue_pv = [&](int t, int j) -> bool {  // O_t += P_t V_j
+        const int s = j % ST;
+        if (!mbar_wait(&bars->p_full[t], j & 1, ctl)) return false;
+        if (!mbar_wait(&bars->v_full[s], (j / ST) & 1, ctl)) return false;
+        tc_fence_after();
+        const uint32_t vbase = sV0 + s * C::kVBytes;
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_f16_ts(tmem + 256 + t * DV, tmem + t * 128 + kk * 8,
+                     make_sw128_desc(vbase + kk * 16 * 128, kBN * 128, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&bars->o_done[t]);
+        return true;
+      };
+      bool ok = mbar_wait(&bars->q_full, 0, ctl);
+      if (ok && n_t[0] > 0) ok = issue_s(0, 0);
+      if (ok && n_t[1] > 0) ok = issue_s(1, 0);
+      for (int j = 0; ok && j < n_kv; ++j) {
+        if (j < n_t[0]) {
+          ok = issue_pv(0, j);
+          if (ok && j + 1 < n_t[0]) ok = issue_s(0, j + 1);
+        }
+        if (ok && j < n_t[1]) ok = issue_pv(1, j);
+        if (!ok) break;
+        mma_commit(&bars->kv_empty[j % ST]);  // K_j, V_j no longer read
+        if (j + 1 < n_t[1]) ok = issue_s(1, j + 1);
+      }
+      mma_commit(&bars->mma_done);  // every MMA issued so far must finish before TMEM is released
+      WaitCtl drain = ctl;
+      drain.deadline_ns = globaltimer_ns() + p.timeout_ns;
+      int dummy = 0;
+      drain.abort_flag = &dummy;
+      mbar_wait(&bars->mma_done, 0, drain);
+    }
+  } else {
+    // ------------------------------------------------ softmax warpgroups
+    const int t = warp >> 2;          // row tile of this warpgroup
+    const int wq = warp & 3;          // TMEM lane quadrant
+    const int r_in = wq * 32 + lane;  // TMEM lane = packed row of the tile
+    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = tmem + lane_base + t * 128;
+    const uint32_t tO = tmem + lane_base + 256 + t * DV;
+    const int tok = rg.tok0 + t * tpt + r_in / p.G;  // of the sequence's new tokens
+    const bool active = r_in < tpt * p.G && tok < sl.count;
+    const bool warp_active = __any_sync(0xffffffffu, active);
+    // rows without a token take no part: whatever they hold stays in their TMEM lane
+    const int lim = active ? limit_of(p, sl, tok) : sl.held;
+    const int lim_w = __shfl_sync(0xffffffffu, lim, 0);  // the least of the warp's
+    const int n_my = n_t[t];
+    const bool fold = p.scale_log2 > 0.0f;  // scale folded into one FFMA (max over raw scores)
+    const float scl = fold ? p.scale_log2 : 1.0f;
+    float m_run = -INFINITY;  // true running max (log2 units, scaled)
+    float m_use = -INFINITY;  // reference max the exponentials are taken against
+    float l = 0.0f;           // sum of exp2(x - m_use)
+    bool ok = true;
+    for (int j = 0; j < n_my; ++j) {
+      if (!warp_wait(&bars->s_full[t], j & 1, ctl)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int kv0 = (rg.j0 + j) * kBN;
+      if (kv0 + kBN > sl.held && (t == 0 || j >= n_t[0])) {
+        // the first user of V_j clears its rows behind the sequence (thread r: row r)
+        const int s = j % ST;
+        if (!warp_wait(&bars->v_full[s], (j / ST) & 1, ctl)) {
+          ok = false;
+          break;
+        }
+        if (kv0 + r_in >= sl.held) {
+#pragma unroll
+          for (int c = 0; c < DV / 64; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(smem + C::kVOff + s * C::kVBytes + c * kBN * 128 + r_in * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      if (warp_active) {
+        uint32_t r[128];
+        SDPA_TMEM_LD32(tS + 0, (r + 0));
+        SDPA_TMEM_LD32(tS + 32, (r + 32));
+        SDPA_TMEM_LD32(tS + 64, (r + 64));
+        SDPA_TMEM_LD32(tS + 96, (r + 96));
+        tmem_wait_ld();
+        if (!fold) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * p.scale_log2);
+        }
+        if (kv0 + kBN > lim_w) {  // some row of the warp does not see the whole tile
+          const int left = max(0, min(kBN, lim - kv0));
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= left) r[c] = __float_as_uint(-INFINITY);
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four independent chains
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mx[q] = fmax3(mx[q], __uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
+        const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scl;
+        m_run = fmaxf(m_run, tmax);
+        float alpha = 1.0f;
+        bool rescale_o = false;
+        if (tmax > m_use + tc::kRescaleThreshold) {
+          alpha = ex2(m_use - m_run);  // 0 when m_use = -inf
+          rescale_o = (j > 0) && (m_use != -INFINITY);
+          m_use = m_run;
+          l *= alpha;
+        }
+        const float nmu = (m_use == -INFINITY) ? 0.0f : -m_use;
+        float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const float p0 = ex2(fmaf(__uint_as_float(r[c]), scl, nmu));
+          const float p1 = ex2(fmaf(__uint_as_float(r[c + 1]), scl, nmu));
+          rs[(c >> 1) & 3] += p0 + p1;
+          r[c / 2] = pack_half2(p0, p1);  // p <= 2^8 enters the product as fp16; the sum l keeps fp32
+        }
+        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        SDPA_TMEM_ST32(tS + 0, (r + 0));
+        SDPA_TMEM_ST32(tS + 32, (r + 32));
+        if (__any_sync(0xffffffffu, rescale_o)) {
+          // O_t holds PV_t(j-1) (committed before S_t(j)); rescale it before PV_t(j)
+          if (!warp_wait(&bars->o_done[t], (j - 1) & 1, ctl)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float a = rescale_o ? alpha : 1.0f;
+#pragma unroll
+          for (int c = 0; c < DV / 32; ++c) {
+            uint32_t o[32];
+            SDPA_TMEM_LD32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            SDPA_TMEM_ST32(tO + c * 32, o);
+          }
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive(&bars->p_full[t]);
+    }
+    // ----------------------------------------------------------- epilogue
+    if (ok && n_my > 0) ok = warp_wait(&bars->o_done[t], (n_my - 1) & 1, ctl);
+    if (ok && warp_active) {
+      tc_fence_after();
+      const float f = m_run == -INFINITY ? 0.0f : ex2(m_use - m_run);
+      const float l_true = l * f;  // relative to the true max
+      const int64_t row = static_cast<int64_t>(sl.begin + tok) * p.H_q + w.head * p.G + r_in % p.G;
+      const int64_t prow = static_cast<int64_t>(w.slot) * (2 * kBM) + t * kBM + r_in;
+      const bool part = w.pieces > 1;
+      const float mul = part ? f : (l_true > kEps ? f / l_true : 0.0f);
+      if (active) {
+        if (part)
+          p.part_ml[prow] = make_float2(m_run, l_true);
+        else
+          p.stats[row] = (m_run == -INFINITY ? kNegInit : m_run * kLn2) + logf(l_true + kEps);
+      }
+#pragma unroll
+      for (int c = 0; c < DV / 32; ++c) {
+        uint32_t o[32];
+        if (n_my > 0) {
+          SDPA_TMEM_LD32(tO + c * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        // a row that saw no key has no sum to scale (its O lane may hold anything)
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = mul == 0.0f ? 0.0f : __uint_as_float(o[e]) * mul;
+        if (active) {
+          if (part) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * DV + c * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+          } else {
+            __half* dst = static_cast<__half*>(p.out) + row * p.D_v + c * 32;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c * 32 + e * 8 < p.D_v)
+                *reinterpret_cast<uint4*>(dst + e * 8) =
+                    make_uint4(pack_half2(x[8 * e], x[8 * e + 1]), pack_half2(x[8 * e + 2], x[8 * e + 3]),
+                               pack_half2(x[8 * e + 4], x[8 * e + 5]), pack_half2(x[8 * e + 6], x[8 * e + 7]));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// Joins the pieces of one item: grid (workspace slots, shares of its rows); a
+// thread adds one float4 column of one row over the pieces.
+template <int DV>
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
+  __shared__ SchedSmem<kMergeThreads> sched;
+  constexpr int CH = DV / 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  Piece w;
+  if (!find_piece<kMergeThreads>(p, blockIdx.x, true, sched, w)) return;
+  if (w.pieces == 1 || w.piece != 0) return;
+  const SeqLens sl = seq_lens(p.view, w.seq);
+  const Range rg = range_of(p, sl, w);
+  const int tpt = kBM / p.G;
+  for (int idx = blockIdx.y * kMergeThreads + threadIdx.x; idx < 2 * kBM * CH; idx += gridDim.y * kMergeThreads) {
+    const int row = idx / CH, c = (idx - row * CH) * 4;
+    const int t = row / kBM, r_in = row - t * kBM;
+    const int tok = rg.tok0 + t * tpt + r_in / p.G;
+    if (r_in >= tpt * p.G || tok >= sl.count) continue;
+    const int64_t first = static_cast<int64_t>(w.slot) * (2 * kBM) + row;
+    float m = -INFINITY;
+    for (int i = 0; i < w.pieces; ++i) m = fmaxf(m, p.part_ml[first + i * 2 * kBM].x);
+    const float u = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < w.pieces; ++i) {
+      const float2 a = p.part_ml[first + i * 2 * kBM];
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (first + i * 2 * kBM) * DV + c);
+      const float f = ex2(a.x - u);
+      l = fmaf(a.y, f, l);
+      acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+    }
+    paged::store_row<__half>(p, static_cast<int64_t>(sl.begin + tok) * p.H_q + w.head * p.G + r_in % p.G, c, acc, m, l);
+  }
+}
+
+}  // namespace paged_tc
+}  // namespace sdpa_b200
