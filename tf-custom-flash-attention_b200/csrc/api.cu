@@ -469,7 +469,7 @@ int fill_view(PagedView& v, const int32_t* page_table, int64_t table_width, cons
   if (seqs < 0 || tokens < 0 || table_width < 0 || num_pages < 0) return SDPA_B200_EINVAL;
   if (seqs >= kIntMax || tokens > kIntMax || table_width > kIntMax || num_pages > kIntMax) return SDPA_B200_EINVAL;
   if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1))) return SDPA_B200_EINVAL;
-  if (table_width * page_size > kIntMax - 65536) return SDPA_B200_EINVAL;
+  if (table_width * page_size > kIntMax - 65536) return SDPA_B200_EINVAL;  // keys are counted in 32 bits
   if (seqs > 0 && (!kv_len || !q_start || (table_width > 0 && !page_table))) return SDPA_B200_EINVAL;
   v.page_table = page_table;
   v.kv_len = kv_len;
@@ -583,7 +583,7 @@ int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void*
   if (tokens == 0 || seqs == 0) return SDPA_B200_OK;
   if (H_q > kIntMax / tokens) return SDPA_B200_EINVAL;  // packed rows are counted in 32 bits
   if (!q || !out || !stats || !aligned16(q) || !aligned16(out) || !stride_ok(dtype, q_stride, H_q * D)) return SDPA_B200_EINVAL;
-  if (num_pages > 0 && (!k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages))) return SDPA_B200_EINVAL;
+  if (num_pages < 1 || !k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages)) return SDPA_B200_EINVAL;
   if (!workspace || !aligned16(workspace) ||
       workspace_bytes < sdpa_b200_paged_workspace_bytes(dtype, tokens, seqs, H_q, H_kv, D, D_v))
     return SDPA_B200_EWORKSPACE;

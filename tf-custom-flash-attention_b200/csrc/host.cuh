@@ -118,6 +118,27 @@ inline bool make_map_rows_f32(CUtensorMap* m, const float* base, int64_t B, int6
   return r == CUDA_SUCCESS || map_failure(static_cast<int>(r), "cuTensorMapEncodeTiled");
 }
 
+// A 4-D map with explicit strides (in elements), for the packed queries and the
+// page pools: 128-byte swizzle, elements of `esize` bytes (2: half, 4: float).
+inline bool make_map_4d(CUtensorMap* m, int esize, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+                        const int (&box)[4]) {
+  auto fn = encode_fn();
+  if (!fn) return map_failure(0, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], e[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) d[i] = static_cast<cuuint64_t>(dims[i]), b[i] = static_cast<cuuint32_t>(box[i]);
+  for (int i = 0; i < 3; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * static_cast<cuuint64_t>(esize);
+  const CUresult r = fn(m, esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+                        const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS || map_failure(static_cast<int>(r), "cuTensorMapEncodeTiled");
+}
+// Pool [pages, page, H_kv, D]: boxes of one 128-byte row segment x 1 head x `rows` rows x 1 page.
+inline bool make_pool_map(CUtensorMap* m, int esize, const void* base, int64_t pages, int64_t page, int64_t H_kv, int64_t D,
+                          int rows) {
+  return make_map_4d(m, esize, base, {D, H_kv, page, pages}, {D, H_kv * D, page * H_kv * D}, {128 / esize, 1, rows, 1});
+}
+
 // Opt a kernel into more than 48 KB of dynamic shared memory, once per device.
 template <typename K>
 inline cudaError_t ensure_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done_mask) {

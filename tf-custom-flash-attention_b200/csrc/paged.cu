@@ -20,47 +20,43 @@ int row_tiles_of(int64_t tokens, int64_t seqs, int64_t group) {
   return mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
 }
 
-int max_ctas() { return 2 * num_sms(); }
-
-// Workspace of the cut items: [ctas][2][rows] sums, (max, sum) pairs, one record a CTA.
+// Workspace of the cut items: [ranges][2][rows] sums, (max, sum) pairs, one record a range.
 struct Layout {
   size_t o, ml, item, bytes;
 };
-Layout layout_of(int ctas, int rows, int db) {
-  const size_t n = static_cast<size_t>(ctas) * 2 * rows;
+template <typename T, int DB, int MT>
+Layout layout_of() {
+  using S = paged::Shape<T, DB, MT>;
+  const size_t ranges = static_cast<size_t>(S::kCtas) * num_sms() * S::kGroups;
+  const size_t n = ranges * 2 * S::kRowsAll;
   Layout l;
   l.o = 0;
-  l.ml = l.o + n * db * sizeof(float);
+  l.ml = l.o + n * DB * sizeof(float);
   l.item = l.ml + n * sizeof(float2);
-  l.bytes = l.item + static_cast<size_t>(ctas) * sizeof(int4);
+  l.bytes = l.item + ranges * sizeof(int4);
   return l;
 }
 
 template <typename T, int DB, int MT>
 int launch_mma_t(paged::Params p, void* workspace, cudaStream_t st, int* launches) {
   static std::atomic<uint64_t> attr_done{0};
+  using S = paged::Shape<T, DB, MT>;
   auto kern = paged::attend_kernel<T, DB, MT>;
-  const size_t smem = sizeof(paged::Smem<DB, MT>) + (sizeof(T) == 4 ? static_cast<size_t>(MT) * (DB / 16) * 4 * 32 * 16 : 0);
-  if (cudaError_t e = ensure_smem(kern, smem, attr_done)) return cuda_failure("shared-memory attribute", e);
-  const int ctas = max_ctas();
-  const Layout l = layout_of(ctas, paged::kRows * MT, DB);
+  if (cudaError_t e = ensure_smem(kern, S::kSmemBytes, attr_done)) return cuda_failure("shared-memory attribute", e);
+  const int ctas = S::kCtas * num_sms();
+  const Layout l = layout_of<T, DB, MT>();
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(w + l.o);
   p.part_ml = reinterpret_cast<float2*>(w + l.ml);
   p.part_item = reinterpret_cast<int4*>(w + l.item);
-  if (int r = launch_tc(kern, ctas, paged::kThreads, smem, st, p)) return r;
+  CUtensorMap mk, mv;
+  const int64_t page = int64_t(1) << p.view.page_shift;
+  if (!make_pool_map(&mk, sizeof(T), p.k_pages, p.view.num_pages, page, p.H_kv, p.D, S::kKeys) ||
+      !make_pool_map(&mv, sizeof(T), p.v_pages, p.view.num_pages, page, p.H_kv, p.D_v, S::kKeys))
+    return SDPA_B200_ECUDA;  // detail recorded by make_map_4d
+  if (int r = launch_tc(kern, ctas, paged::kThreads, S::kSmemBytes, st, mk, mv, p)) return r;
   ++*launches;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), paged::kRows * MT * (DB / 4) / paged::kThreads);
-  cfg.blockDim = dim3(paged::kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged::merge_kernel<T, DB, MT>, p);
-  if (e != cudaSuccess) return cuda_failure("kernel launch", e);
+  if (int r = launch_tc(paged::merge_kernel<T, DB, MT>, ctas * S::kGroups, paged::kMergeThreads, 0, st, p)) return r;
   ++*launches;
   return SDPA_B200_OK;
 }
@@ -70,6 +66,11 @@ int launch_mma(const paged::Params& p, void* ws, int mt, cudaStream_t st, int* l
   return mt == 1   ? launch_mma_t<T, DB, 1>(p, ws, st, launches)
          : mt == 2 ? launch_mma_t<T, DB, 2>(p, ws, st, launches)
                    : launch_mma_t<T, DB, 4>(p, ws, st, launches);
+}
+
+template <typename T, int DB>
+size_t bytes_of(int mt) {
+  return mt == 1 ? layout_of<T, DB, 1>().bytes : mt == 2 ? layout_of<T, DB, 2>().bytes : layout_of<T, DB, 4>().bytes;
 }
 
 }  // namespace
@@ -85,7 +86,9 @@ size_t sdpa_b200::paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs,
                                         int64_t D_v) {
   if (use_tc(dtype, tokens, seqs, H_q / H_kv)) return paged_tc_workspace_bytes(static_cast<int>(D_v));
   const int mt = row_tiles_of(tokens, seqs, H_q / H_kv);
-  return layout_of(max_ctas(), paged::kRows * mt, bucket_of(static_cast<int>(D), static_cast<int>(D_v))).bytes;
+  const bool small = bucket_of(static_cast<int>(D), static_cast<int>(D_v)) == 64;
+  if (dtype == SDPA_B200_F16) return small ? bytes_of<__half, 64>(mt) : bytes_of<__half, 128>(mt);
+  return small ? bytes_of<float, 64>(mt) : bytes_of<float, 128>(mt);
 }
 
 int sdpa_b200::launch_paged_sdpa(int dtype, paged::Params p, void* workspace, cudaStream_t st, int* launches) {

@@ -11,32 +11,34 @@
 // fp32): 16 rows are a tenth of a tcgen05 tile, and its operands would have to
 // pass through shared memory and TMEM, while these take them from registers.
 //
-// Register operands straight from global memory: a matrix product may take its
-// inner index in any order as long as both operands agree.  A lane (g = lane/4,
-// t = lane%4) therefore reads 16-byte words, K[key g][32i + 8t ..], and uses
-// their four 32-bit parts as the B operands of two instructions, with Q's A
-// operands laid out the same way; V[key 2t][64i + 8g ..] likewise, neighbouring
-// keys joined by byte permutes.  No shared memory, no barrier in the loop, and
-// every warp streams on its own: block of kKeys keys = K and V words of one
-// block in flight while the previous is computed.
+// Every warp streams alone: TMA boxes of one block of keys (16 fp16, 8 fp32;
+// always inside one page) go to the warp's own ring of kStages blocks in shared
+// memory, 128-byte swizzled, so the matrix operands come out of it without
+// bank conflicts (ldmatrix; for fp32 values 16-byte loads, four output columns
+// a word), and no barrier of the CTA stands in the loop.  (Operands copied lane
+// by lane, with plain loads or cp.async, took 450 instructions a block of 16
+// keys and 196 / 243 us for 16 x 32768 keys x 4 heads; this takes about 170.)
 //
-// Work: every (sequence, KV head, row tile) item has ceil(held / 64) tiles of
-// 64 keys; the tiles of all items, in order, are cut into equal ranges, one per
-// CTA, so long and short sequences load the device evenly.  An item that lies
-// in one CTA is finished there; one that is cut leaves partial sums (at most two
-// a CTA) that merge_kernel joins.
+// Work: every (sequence, KV head, row tile) item has ceil(held / 32) tiles of
+// 32 keys; the tiles of all items, in order, are cut into equal ranges, one a
+// warp (with more than 16 packed rows a sequence, one a group of 2 or 4 warps
+// with a row tile each), so long and short sequences load the device evenly.
+// An item that lies in one range is finished there; one that is cut leaves
+// partial sums, at most two a range, that merge_kernel joins.
 #pragma once
 #include "common.cuh"
+#include "fwd_tc.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
 
 namespace sdpa_b200 {
 namespace paged {
 
-constexpr int kTile = 64;       // keys of one unit of work
+constexpr int kTile = 32;       // keys of one unit of work
 constexpr int kRows = 16;       // packed query rows of one matrix tile
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMergeThreads = 256;
 
 struct Params {
   const void* q;
@@ -50,9 +52,10 @@ struct Params {
   float scale_log2;
   int causal;
   // workspace
-  float* part_o;          // [ctas, 2, rows, DB] unnormalised sums
-  float2* part_ml;        // [ctas, 2, rows] (max, sum), log2 units
-  int4* part_item;        // [ctas] (sequence, head, row tile, CTAs after this one that hold the rest; -1: none)
+  float* part_o;          // [ranges, 2, rows, DB] unnormalised sums
+  float2* part_ml;        // [ranges, 2, rows] (max, sum), log2 units
+  int4* part_item;        // [ranges] (sequence, head, row tile, ranges after this one that hold the rest; -1: none)
+  int* part_slots;        // tcgen05 kernel: slots of the call (its part_item: [slots] items)
   int sms;                // SMs of the device
   uint64_t timeout_ns;
 };
@@ -76,136 +79,171 @@ __device__ __forceinline__ void split_fast(float x, uint32_t& hi, uint32_t& lo) 
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
+__device__ __forceinline__ void split_fast(const uint4& x, uint4& hi, uint4& lo) {
+  split_fast(__uint_as_float(x.x), hi.x, lo.x);
+  split_fast(__uint_as_float(x.y), hi.y, lo.y);
+  split_fast(__uint_as_float(x.z), hi.z, lo.z);
+  split_fast(__uint_as_float(x.w), hi.w, lo.w);
+}
 
-// Per type: keys of a warp's block and 16-byte words of one row.
-template <typename T>
-struct Kind;
-template <>
-struct Kind<__half> {
-  static constexpr int kKeys = 16;
-};
-template <>
-struct Kind<float> {
-  static constexpr int kKeys = 8;
-};
-
-// 16 bytes of a read-only row, kept out of L1 unless several warps of the CTA
-// read the same rows.
-template <bool SHARED_ROWS>
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  if (SHARED_ROWS)
-    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
-  return r;
+// Four 8 x 8 matrices of 16-bit elements (or 8 x 4 of 32-bit ones); lane i
+// gives the row address of matrix i / 8, row i % 8.
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 __device__ __forceinline__ int row_tiles(const Params& p, const SeqLens& s, int rows) {
   return static_cast<int>((static_cast<int64_t>(s.count) * p.G + rows - 1) / rows);
 }
 __device__ __forceinline__ int key_tiles(const SeqLens& s) { return s.held > 0 ? (s.held + kTile - 1) / kTile : 1; }
-// Tiles of all items of sequence n.
-__device__ __forceinline__ int64_t seq_work(const Params& p, int n, int rows) {
-  const SeqLens s = seq_lens(p.view, n);
-  return static_cast<int64_t>(row_tiles(p, s, rows)) * p.H_kv * key_tiles(s);
-}
 
-template <int DB, int MT>
-struct Smem {
-  static constexpr int kOStride = DB + 4;
-  float o[kWarps][kRows][kOStride];
-  float m[kWarps][kRows], l[kWarps][kRows];
+// Shapes of one instantiation.  DB: feature bucket; MT: row tiles (warps) of a
+// group, which shares one ring.
+template <typename T, int DB, int MT>
+struct Shape {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kKeys = kHalf ? 16 : 8;              // keys of a block
+  static constexpr int kBoxes = DB * static_cast<int>(sizeof(T)) / 128;  // 128-byte column boxes of K, and of V
+  static constexpr int kBoxBytes = kKeys * 128;
+  static constexpr int kStageBytes = 2 * kBoxes * kBoxBytes;  // 8 KB at DB = 128
+  static constexpr int kCtas = DB == 64 ? 3 : 2;            // resident CTAs an SM
+  static constexpr int kStages = (DB == 64 ? (kHalf ? 4 : 3) : (kHalf ? 3 : 2)) * MT;
+  static constexpr int kGroups = kWarps / MT;               // ranges of a CTA
+  static constexpr int kQBytes = kHalf ? 0 : DB / 8 * 512;  // a warp's low parts of Q (fp32)
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kSmemBytes = kGroups * kRingBytes + kWarps * kQBytes + 1024;  // + alignment slack
+  static constexpr int kRowsAll = kRows * MT;
 };
 
-// Four columns of one output row from its sums (and, at column 0, its stats):
-// the op's row rule, stats = max + ln(l + 1e-6), rows that saw no key are zero.
+// One output row's four columns from its sums (and, where asked, its stats):
+// stats = max + ln(l + 1e-6); a row that saw no key is zero.
+__device__ __forceinline__ float row_stats(float m, float l) {
+  return (m == -INFINITY ? kNegInit : m * kLn2) + logf(l + kEps);
+}
+__device__ __forceinline__ float row_scale(float l) { return l > kEps ? 1.0f / l : 0.0f; }
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float x, float y, float z, float w) {
+  if (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(x, y), pack_half2(z, w));
+  else
+    *reinterpret_cast<float4*>(dst) = make_float4(x, y, z, w);
+}
 template <typename T>
 __device__ __forceinline__ void store_row(const Params& p, int64_t row, int c, const float4& acc, float m, float l) {
-  const float inv = l > kEps ? 1.0f / l : 0.0f;
-  if (c == 0) p.stats[row] = (m == -INFINITY ? kNegInit : m * kLn2) + logf(l + kEps);
-  if (c >= p.D_v) return;
-  T* dst = static_cast<T*>(p.out) + row * p.D_v + c;
-  if (sizeof(T) == 2) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
-  } else {
-    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-  }
+  const float inv = row_scale(l);
+  if (c == 0) p.stats[row] = row_stats(m, l);
+  if (c < p.D_v) store4<T>(static_cast<T*>(p.out) + row * p.D_v + c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-// MT row tiles of 16 by 4 / MT shares of the keys: with more than one row tile
-// the warps of a share read the same rows (the second reading hits L1).
+// (m, l, acc) += a piece's (max, sum) and sums.
+__device__ __forceinline__ void join(float& m, float& l, float4& acc, const float2& ml, const float4& x) {
+  const float up = fmaxf(m, ml.x), u = up == -INFINITY ? 0.0f : up;
+  const float f = ex2(m - u), w = ex2(ml.x - u);
+  m = up;
+  l = fmaf(ml.y, w, l * f);
+  acc.x = fmaf(x.x, w, acc.x * f), acc.y = fmaf(x.y, w, acc.y * f);
+  acc.z = fmaf(x.z, w, acc.z * f), acc.w = fmaf(x.w, w, acc.w * f);
+}
+
 template <typename T, int DB, int MT>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
-  constexpr int KS = kWarps / MT;
-  constexpr int KEYS = Kind<T>::kKeys;
-  constexpr bool HALF = sizeof(T) == 2;
-  constexpr int KW = HALF ? DB / 32 : DB / 16;        // K words a lane reads of one key
-  constexpr int KN = KEYS / 8;                        // keys a lane reads K of
-  constexpr int VW = HALF ? DB / 64 : DB / 32;        // V words a lane reads of one key
-  constexpr int VN = HALF ? 4 : 2;                    // keys a lane reads V of
-  constexpr int NO = DB / 8;                          // output column tiles
-  constexpr int ROWS = kRows * MT;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  Smem<DB, MT>& sm = *reinterpret_cast<Smem<DB, MT>*>(smem_raw);
-  // fp32: Q's operands, hi and lo, as [row tile][word][4][lane] float4
-  uint4* const sq = reinterpret_cast<uint4*>(smem_raw + sizeof(Smem<DB, MT>));
-  __shared__ int64_t s_sum[kWarps];
-  __shared__ int64_t s_base;
-  __shared__ int s_seq;
+__global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
+    attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  using S = Shape<T, DB, MT>;
+  constexpr bool HALF = S::kHalf;
+  constexpr int KEYS = S::kKeys, ST = S::kStages, BX = S::kBoxes;
+  constexpr int KN = KEYS / 8;                 // score column tiles of a block
+  constexpr int KS = HALF ? DB / 16 : DB / 8;  // inner steps of Q K^T
+  constexpr int NO = DB / 8;                   // output column tiles
+  constexpr int ROWS = S::kRowsAll;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = tc::align1024(smem_raw);
+  __shared__ uint64_t s_full[S::kGroups * ST], s_empty[S::kGroups * ST];
+  __shared__ int64_t s_warp[kWarps];
+  __shared__ int64_t s_before[kThreads];  // tiles before thread i's sequences
+  __shared__ int s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int mt = warp % MT, ks = warp / MT;
+  const int mt = warp % MT, group = warp / MT;
   const int g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = smem + group * S::kRingBytes;
+  uint64_t* const full = s_full + group * ST;
+  uint64_t* const empty = s_empty + group * ST;  // (used by groups of several warps)
+  uint4* const q_lo = reinterpret_cast<uint4*>(smem + S::kGroups * S::kRingBytes + warp * S::kQBytes) + lane;  // fp32
+  if (tid == 0) {
+    for (int i = 0; i < S::kGroups * ST; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], MT);
+    }
+    s_abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
   pdl_launch_dependents();
   pdl_wait();
+  WaitCtl ctl;
+  ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;
+  ctl.abort_flag = &s_abort;
 
-  // ---- this CTA's range of tiles
+  // ---- this group's range of tiles
   const int per = (p.view.seqs + kThreads - 1) / kThreads;
   int64_t mine = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < p.view.seqs) mine += seq_work(p, tid * per + i, ROWS);
+  for (int n = tid * per; n < min(p.view.seqs, (tid + 1) * per); ++n) {
+    const SeqLens s = seq_lens(p.view, n);
+    mine += static_cast<int64_t>(row_tiles(p, s, ROWS)) * key_tiles(s);
+  }
+  mine *= p.H_kv;
   int64_t incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += up;
   }
-  if (lane == 31) s_sum[warp] = incl;
+  if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
   int64_t before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
   }
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-  if (tid == 0) p.part_item[blockIdx.x] = make_int4(0, 0, 0, -1);
-  if (blockIdx.x >= ctas) return;
-  const int64_t w0 = total * blockIdx.x / ctas, w1 = total * (blockIdx.x + 1) / ctas;
-  const int64_t excl = before + incl - mine;
-  if (excl <= w0 && w0 < excl + mine) {
-    int64_t base = excl;
-    int n = tid * per;
-    for (;; ++n) {
-      const int64_t s = seq_work(p, n, ROWS);
-      if (w0 < base + s) break;
-      base += s;
-    }
-    s_seq = n;
-    s_base = base;
-  }
+  s_before[tid] = before + incl - mine;
   __syncthreads();
-  int n = s_seq;
-  int64_t base = s_base;
+  const int64_t range = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(gridDim.x) * group;
+  const int64_t ranges = min(static_cast<int64_t>(gridDim.x) * S::kGroups, total);
+  if (range >= ranges) {
+    if (mt == 0 && lane == 0) p.part_item[range] = make_int4(0, 0, 0, -1);
+    return;
+  }
+  const int64_t w0 = total * range / ranges, w1 = total * (range + 1) / ranges;
+  // the last thread whose sequences begin at or before w0 (a chunk without work begins where the next does)
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) c += __popc(__ballot_sync(0xffffffffu, s_before[i * 32 + lane] <= w0));
+  int n = (c - 1) * per;
+  int64_t base = s_before[c - 1];
+  int4 record = make_int4(0, 0, 0, -1);
 
-  const int64_t k_row = static_cast<int64_t>(p.H_kv) * p.D, v_row = static_cast<int64_t>(p.H_kv) * p.D_v;
   const int page_shift = p.view.page_shift, page_mask = (1 << page_shift) - 1;
-  const bool whole = p.D == DB && p.D_v == DB;
+  // this lane's row and 16-byte chunk in the ldmatrix loads of K and V (chunk ^ row % 8: the swizzle)
+  const int sw = lane & 7, mi = lane >> 3;
+  const uint32_t k_off = HALF ? ((mi >> 1) * 8 + sw) * 128 : sw * 128;
+  const int k_chunk = HALF ? (mi & 1) : mi;
+  const uint32_t v_off = HALF ? ((mi & 1) * 8 + sw) * 128 : 0;
+  const int v_chunk = mi >> 1;
+  int done = 0;  // blocks this group has taken through its ring
+  bool ok = true;
 
-  for (int64_t w = w0; w < w1;) {
+  for (int64_t w = w0; w < w1 && ok;) {
     const SeqLens sl = seq_lens(p.view, n);
     const int rt = row_tiles(p, sl, ROWS), nt = key_tiles(sl);
     const int64_t work = static_cast<int64_t>(rt) * p.H_kv * nt;
@@ -220,6 +258,48 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
     const int head = static_cast<int>(item / rt), rtile = static_cast<int>(item - static_cast<int64_t>(head) * rt);
     const int tiles = static_cast<int>(min(static_cast<int64_t>(nt - tile0), w1 - w));
 
+    // ---- the blocks of keys, and their copies
+    const int blk0 = tile0 * (kTile / KEYS);
+    const int blocks = (min((tile0 + tiles) * kTile, sl.held) + KEYS - 1) / KEYS - blk0;
+    // pages of 32 blocks, one a lane, read a batch ahead
+    auto pages_from = [&](int i) {
+      return i + lane < blocks ? page_of(p.view, n, ((blk0 + i + lane) * KEYS) >> page_shift) : -1;
+    };
+    int pages = -1, pages_next = -1;
+    if (mt == 0) pages = pages_from(0), pages_next = pages_from(32);
+    // Block i to its stage (whole warp; the group's first).  Features behind D
+    // and pages outside the pool (-1) read as zeros.
+    auto copy_block = [&](int i) {
+      if (i > 0 && (i & 31) == 0) {
+        pages = pages_next;
+        pages_next = pages_from(i + 32);
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+      if (lane == 0) {
+        const int stage = (done + i) % ST;
+        const int row = ((blk0 + i) * KEYS) & page_mask;
+        uint8_t* const dst = ring + stage * S::kStageBytes;
+        mbar_expect_tx(&full[stage], S::kStageBytes);
+#pragma unroll
+        for (int x = 0; x < BX; ++x)
+          tma_load_4d(dst + x * S::kBoxBytes, &tm_k, x * (128 / static_cast<int>(sizeof(T))), head, row, page, &full[stage]);
+#pragma unroll
+        for (int x = 0; x < BX; ++x)
+          tma_load_4d(dst + (BX + x) * S::kBoxBytes, &tm_v, x * (128 / static_cast<int>(sizeof(T))), head, row, page,
+                      &full[stage]);
+      }
+    };
+    int copied = 0;
+    if (mt == 0)
+      for (; copied < min(ST, blocks); ++copied) {
+        // a group of several warps: all of them have left the stage's last block
+        if (MT > 1 && !tc::warp_wait(&empty[(done + copied) % ST], (((done + copied) / ST) & 1) ^ 1, ctl)) {
+          ok = false;
+          break;
+        }
+        copy_block(copied);
+      }
+
     // ---- rows of this warp
     const int total_rows = sl.count * p.G;
     const int r0 = (rtile * MT + mt) * kRows;
@@ -232,110 +312,50 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
     const int lim_0 = p.causal ? min(sl.held, shift + r0 / p.G + 1) : sl.held;  // the least of the warp's
     const T* qa = static_cast<const T*>(p.q) + (sl.begin + ra / p.G) * p.q_stride + (head * p.G + ra % p.G) * p.D;
     const T* qb = static_cast<const T*>(p.q) + (sl.begin + rb / p.G) * p.q_stride + (head * p.G + rb % p.G) * p.D;
-    uint4 qf[HALF ? 2 * KW : 1];
-    if (HALF) {
+    // A operands: (row g, k t) (row g+8, k t) (row g, k t') (row g+8, k t'); k t is a pair of halves or one float
+    uint32_t qf[KS][4];
 #pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        const int d = 32 * i + 8 * t;
-        qf[2 * i] = va && d < p.D ? ldg16<true>(qa + d) : make_uint4(0, 0, 0, 0);
-        qf[2 * i + 1] = vb && d < p.D ? ldg16<true>(qb + d) : make_uint4(0, 0, 0, 0);
-      }
-    } else {
-      __syncthreads();  // the previous item's readers are done
-      if (ks == 0) {
+    for (int i = 0; i < KS; ++i) {
+      const int d0 = HALF ? 16 * i + 2 * t : 8 * i + t, d1 = d0 + (HALF ? 8 : 4);
+      qf[i][0] = va && d0 < p.D ? __ldg(reinterpret_cast<const uint32_t*>(qa + d0)) : 0u;
+      qf[i][1] = vb && d0 < p.D ? __ldg(reinterpret_cast<const uint32_t*>(qb + d0)) : 0u;
+      qf[i][2] = va && d1 < p.D ? __ldg(reinterpret_cast<const uint32_t*>(qa + d1)) : 0u;
+      qf[i][3] = vb && d1 < p.D ? __ldg(reinterpret_cast<const uint32_t*>(qb + d1)) : 0u;
+    }
+    if (!HALF) {
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          const int d = 16 * i + 4 * t;
-          const uint4 a = va && d < p.D ? ldg16<true>(qa + d) : make_uint4(0, 0, 0, 0);
-          const uint4 b = vb && d < p.D ? ldg16<true>(qb + d) : make_uint4(0, 0, 0, 0);
-          uint4 ah, al, bh, bl;
-          split_fast(__uint_as_float(a.x), ah.x, al.x), split_fast(__uint_as_float(a.y), ah.y, al.y);
-          split_fast(__uint_as_float(a.z), ah.z, al.z), split_fast(__uint_as_float(a.w), ah.w, al.w);
-          split_fast(__uint_as_float(b.x), bh.x, bl.x), split_fast(__uint_as_float(b.y), bh.y, bl.y);
-          split_fast(__uint_as_float(b.z), bh.z, bl.z), split_fast(__uint_as_float(b.w), bh.w, bl.w);
-          // the operand order of the instruction: (row g, k t) (row g+8, k t) (row g, k t+4) (row g+8, k t+4)
-          uint4* dst = sq + ((mt * KW + i) * 4) * 32 + lane;
-          dst[0] = make_uint4(ah.x, bh.x, ah.y, bh.y);
-          dst[32] = make_uint4(ah.z, bh.z, ah.w, bh.w);
-          dst[64] = make_uint4(al.x, bl.x, al.y, bl.y);
-          dst[96] = make_uint4(al.z, bl.z, al.w, bl.w);
-        }
+      for (int i = 0; i < KS; ++i) {
+        uint32_t lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(qf[i][e]), qf[i][e], lo[e]);
+        q_lo[i * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      __syncthreads();
     }
 
-    // ---- the warp's blocks of keys
-    const int blk0 = tile0 * (kTile / KEYS) + ks;
-    const int blk1 = (min((tile0 + tiles) * kTile, sl.held) + KEYS - 1) / KEYS;
     float o[NO][4];
 #pragma unroll
     for (int i = 0; i < NO; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.0f, l_b = 0.0f;
-    uint4 kf[KN][KW], vf[VN][VW];
-    const T* const kp = static_cast<const T*>(p.k_pages) + static_cast<int64_t>(head) * p.D;
-    const T* const vp = static_cast<const T*>(p.v_pages) + static_cast<int64_t>(head) * p.D_v;
 
-    // pages of the next 32 blocks, one a lane, read a batch ahead
-    auto pages_from = [&](int blk) {
-      const int key = (blk + lane * KS) * KEYS;
-      return key < sl.held && blk + lane * KS < blk1 ? page_of(p.view, n, key >> page_shift) : -1;
-    };
-    auto load_k = [&](int blk, int page) {
-      const int key = blk * KEYS;
-      const T* row = kp + ((static_cast<int64_t>(page) << page_shift) + (key & page_mask)) * k_row;
-      if (whole && page >= 0 && key + KEYS <= sl.held) {
-#pragma unroll
-        for (int a = 0; a < KN; ++a)
-#pragma unroll
-          for (int i = 0; i < KW; ++i)
-            kf[a][i] = ldg16<(MT > 1)>(row + (8 * a + g) * k_row + (HALF ? 32 * i + 8 * t : 16 * i + 4 * t));
-      } else {
-#pragma unroll
-        for (int a = 0; a < KN; ++a)
-#pragma unroll
-          for (int i = 0; i < KW; ++i) {
-            const int d = HALF ? 32 * i + 8 * t : 16 * i + 4 * t;
-            kf[a][i] = make_uint4(0, 0, 0, 0);
-            if (page >= 0 && key + 8 * a + g < sl.held && d < p.D) kf[a][i] = ldg16<(MT > 1)>(row + (8 * a + g) * k_row + d);
-          }
+    for (int i = 0; ok && i < blocks; ++i) {
+      const int key0 = (blk0 + i) * KEYS;
+      const int stage = (done + i) % ST;
+      uint8_t* const at = ring + stage * S::kStageBytes;
+      const uint32_t k_at = smem_u32(at), v_at = k_at + BX * S::kBoxBytes;
+      if (!tc::warp_wait(&full[stage], ((done + i) / ST) & 1, ctl)) {
+        ok = false;
+        break;
       }
-    };
-    auto load_v = [&](int blk, int page) {
-      const int key = blk * KEYS;
-      const T* row = vp + ((static_cast<int64_t>(page) << page_shift) + (key & page_mask)) * v_row;
-      if (whole && page >= 0 && key + KEYS <= sl.held) {
-#pragma unroll
-        for (int a = 0; a < VN; ++a)
-#pragma unroll
-          for (int i = 0; i < VW; ++i)
-            vf[a][i] = ldg16<(MT > 1)>(row + (8 * (a >> 1) + 2 * t + (a & 1)) * v_row + (HALF ? 64 * i + 8 * g : 32 * i + 4 * g));
-      } else {  // rows behind the sequence read as zeros: whatever the pool holds there stays out of the sums
-#pragma unroll
-        for (int a = 0; a < VN; ++a)
-#pragma unroll
-          for (int i = 0; i < VW; ++i) {
-            const int d = HALF ? 64 * i + 8 * g : 32 * i + 4 * g, r = 8 * (a >> 1) + 2 * t + (a & 1);
-            vf[a][i] = make_uint4(0, 0, 0, 0);
-            if (page >= 0 && key + r < sl.held && d < p.D_v) vf[a][i] = ldg16<(MT > 1)>(row + r * v_row + d);
-          }
+      if (key0 + KEYS > sl.held) {
+        // V rows behind the sequence count as zeros: whatever the pool holds there stays out of the sums
+        for (int x = lane; x < BX * KEYS * 8; x += 32)
+          if (key0 + (x >> 3) % KEYS >= sl.held)
+            *reinterpret_cast<uint4*>(at + BX * S::kBoxBytes + x * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // before the stage's next copy
+        __syncwarp();
       }
-    };
-
-    int pages = pages_from(blk0), pages_next = pages_from(blk0 + 32 * KS);
-    int page = __shfl_sync(0xffffffffu, pages, 0);
-    if (blk0 < blk1) load_k(blk0, page), load_v(blk0, page);
-    int it = 0;
-    for (int blk = blk0; blk < blk1; blk += KS) {
-      ++it;
-      if ((it & 31) == 0) {
-        pages = pages_next;
-        pages_next = pages_from(blk + KS + 32 * KS);
-      }
-      const int page_n = __shfl_sync(0xffffffffu, pages, it & 31);
-      const bool more = blk + KS < blk1;
-      const int key0 = blk * KEYS;
       // S = Q K^T
       float s[KN][4];
 #pragma unroll
@@ -344,35 +364,31 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         for (int e = 0; e < 4; ++e) s[a][e] = 0.0f;
       if (HALF) {
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          const uint32_t a0[4] = {qf[2 * i].x, qf[2 * i + 1].x, qf[2 * i].y, qf[2 * i + 1].y};
-          const uint32_t a1[4] = {qf[2 * i].z, qf[2 * i + 1].z, qf[2 * i].w, qf[2 * i + 1].w};
-#pragma unroll
-          for (int a = 0; a < KN; ++a) {
-            mma_16816(s[a], a0, kf[a][i].x, kf[a][i].y);
-            mma_16816(s[a], a1, kf[a][i].z, kf[a][i].w);
-          }
+        for (int k = 0; k < KS; ++k) {
+          uint32_t b[4];  // keys 0-7 and 8-15, two operands each
+          ldmatrix4(k_at + (k >> 2) * S::kBoxBytes + k_off + (((2 * (k & 3) + k_chunk) ^ sw) << 4), b);
+          mma_16816(s[0], qf[k], b[0], b[1]);
+          mma_16816(s[KN - 1], qf[k], b[2], b[3]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          const uint4* src = sq + ((mt * KW + i) * 4) * 32 + lane;
-          const uint4 h0 = src[0], h1 = src[32], l0 = src[64], l1 = src[96];
-          uint32_t bh[4], bl[4];
-          split_fast(__uint_as_float(kf[0][i].x), bh[0], bl[0]), split_fast(__uint_as_float(kf[0][i].y), bh[1], bl[1]);
-          split_fast(__uint_as_float(kf[0][i].z), bh[2], bl[2]), split_fast(__uint_as_float(kf[0][i].w), bh[3], bl[3]);
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t b[4], bl[4];  // two inner steps, two operands each
+          ldmatrix4(k_at + (k >> 2) * S::kBoxBytes + k_off + (((2 * (k & 3) + k_chunk) ^ sw) << 4), b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(b[e]), b[e], bl[e]);
+          const uint4 l0 = q_lo[k * 32], l1 = q_lo[(k + 1) * 32];
           float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short sums on the tensor cores, joined in fp32
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&l0), bh[0], bh[1]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&l1), bh[2], bh[3]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&h0), bl[0], bl[1]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&h1), bl[2], bl[3]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&h0), bh[0], bh[1]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&h1), bh[2], bh[3]);
+          mma_1688(part, reinterpret_cast<const uint32_t*>(&l0), b[0], b[1]);
+          mma_1688(part, reinterpret_cast<const uint32_t*>(&l1), b[2], b[3]);
+          mma_1688(part, qf[k], bl[0], bl[1]);
+          mma_1688(part, qf[k + 1], bl[2], bl[3]);
+          mma_1688(part, qf[k], b[0], b[1]);
+          mma_1688(part, qf[k + 1], b[2], b[3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[0][e] += part[e];
         }
       }
-      if (more) load_k(blk + KS, page_n);
       // online softmax in log2 units
       float mx_a = m_a, mx_b = m_b;
 #pragma unroll
@@ -398,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         l_a *= fa;
         l_b *= fb;
 #pragma unroll
-        for (int i = 0; i < NO; ++i) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
+        for (int x = 0; x < NO; ++x) o[x][0] *= fa, o[x][1] *= fa, o[x][2] *= fb, o[x][3] *= fb;
         m_a = mx_a;
         m_b = mx_b;
       }
@@ -417,139 +433,160 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         const uint32_t pa[4] = {pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]),
                                 pack_half2(s[KN - 1][0], s[KN - 1][1]), pack_half2(s[KN - 1][2], s[KN - 1][3])};
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
-          const uint32_t* r0v = reinterpret_cast<const uint32_t*>(&vf[0][i]);
-          const uint32_t* r1v = reinterpret_cast<const uint32_t*>(&vf[1][i]);
-          const uint32_t* r2v = reinterpret_cast<const uint32_t*>(&vf[VN - 2][i]);
-          const uint32_t* r3v = reinterpret_cast<const uint32_t*>(&vf[VN - 1][i]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-            mma_16816(o[8 * i + j], pa, __byte_perm(r0v[j >> 1], r1v[j >> 1], sel), __byte_perm(r2v[j >> 1], r3v[j >> 1], sel));
-          }
+        for (int x = 0; x < NO; x += 2) {
+          uint32_t b[4];  // two column tiles, keys 0-7 and 8-15 each
+          ldmatrix4_trans(v_at + (x >> 3) * S::kBoxBytes + v_off + ((((x & 7) + v_chunk) ^ sw) << 4), b);
+          mma_16816(o[x], pa, b[0], b[1]);
+          mma_16816(o[x + 1], pa, b[2], b[3]);
         }
-      } else {  // inner index t <-> key 2t, t + 4 <-> key 2t + 1
+      } else {  // inner index t <-> key 2t, t + 4 <-> key 2t + 1; word g of a box row: column g of four tiles
         uint32_t ph[4], pl[4];
         split_fast(s[0][0], ph[0], pl[0]), split_fast(s[0][2], ph[1], pl[1]);
         split_fast(s[0][1], ph[2], pl[2]), split_fast(s[0][3], ph[3], pl[3]);
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
-          const uint32_t* r0v = reinterpret_cast<const uint32_t*>(&vf[0][i]);
-          const uint32_t* r1v = reinterpret_cast<const uint32_t*>(&vf[1][i]);
+        for (int x = 0; x < BX; ++x) {
+          const uint8_t* box = at + (BX + x) * S::kBoxBytes;
+          uint4 h0, l0, h1, l1;
+          split_fast(*reinterpret_cast<const uint4*>(box + (2 * t) * 128 + ((g ^ (2 * t)) << 4)), h0, l0);
+          split_fast(*reinterpret_cast<const uint4*>(box + (2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4)), h1, l1);
+          const uint32_t *xh0 = reinterpret_cast<const uint32_t*>(&h0), *xh1 = reinterpret_cast<const uint32_t*>(&h1);
+          const uint32_t *xl0 = reinterpret_cast<const uint32_t*>(&l0), *xl1 = reinterpret_cast<const uint32_t*>(&l1);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint32_t h0, h1, l0, l1;
-            split_fast(__uint_as_float(r0v[j]), h0, l0), split_fast(__uint_as_float(r1v[j]), h1, l1);
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_1688(part, pl, h0, h1);
-            mma_1688(part, ph, l0, l1);
-            mma_1688(part, ph, h0, h1);
+            mma_1688(part, pl, xh0[j], xh1[j]);
+            mma_1688(part, ph, xl0[j], xl1[j]);
+            mma_1688(part, ph, xh0[j], xh1[j]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * i + j][e] += part[e];
+            for (int e = 0; e < 4; ++e) o[4 * x + j][e] += part[e];
           }
         }
       }
-      if (more) load_v(blk + KS, page_n);
+      __syncwarp();  // every lane has left the stage
+      if (MT > 1 && lane == 0) mbar_arrive(&empty[stage]);
+      if (mt == 0 && copied < blocks) {
+        if (MT > 1 && !tc::warp_wait(&empty[stage], ((done + i) / ST) & 1, ctl)) {
+          ok = false;
+          break;
+        }
+        copy_block(copied++);
+      }
     }
+    if (!ok) {  // let copies in flight land before the CTA exits
+      if (mt == 0 && lane == 0) {
+        WaitCtl drain = ctl;
+        drain.deadline_ns = globaltimer_ns() + p.timeout_ns;
+        int dummy = 0;
+        drain.abort_flag = &dummy;
+        for (int i = max(0, copied - ST); i < copied; ++i) mbar_wait(&full[(done + i) % ST], ((done + i) / ST) & 1, drain);
+      }
+      break;
+    }
+    done += blocks;
 
-    // ---- join the key shares
+    // ---- the item's sums, or this range's part of them
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
-    __syncthreads();  // the previous item's sums have been read
-    if (t == 0) {
-      sm.m[warp][g] = m_a, sm.m[warp][g + 8] = m_b;
-      sm.l[warp][g] = l_a, sm.l[warp][g + 8] = l_b;
-    }
-    // column n = 2t + (e & 1) of output tile (i, j) is feature W i + (W / 8) n + j, W = 64 (fp16), 32 (fp32)
-    constexpr int J = HALF ? 8 : 4;
-#pragma unroll
-    for (int i = 0; i < VW; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int j = 0; j < J; j += 4) {
-          const int col = i * J * 8 + J * (2 * t + e) + j;
-          *reinterpret_cast<float4*>(&sm.o[warp][g][col]) =
-              make_float4(o[J * i + j][e], o[J * i + j + 1][e], o[J * i + j + 2][e], o[J * i + j + 3][e]);
-          *reinterpret_cast<float4*>(&sm.o[warp][g + 8][col]) =
-              make_float4(o[J * i + j][2 + e], o[J * i + j + 1][2 + e], o[J * i + j + 2][2 + e], o[J * i + j + 3][2 + e]);
-        }
-    __syncthreads();
     const bool complete = tile0 == 0 && tiles == nt;
-    const int slot = tile0 == 0 ? 1 : 0;  // 0: the item began before this CTA
-    if (!complete && slot == 1 && tid == 0) {
+    const int slot = tile0 == 0 ? 1 : 0;  // 0: the item began before this range
+    if (!complete && slot == 1) {
       const int64_t last = base + (item + 1) * nt;  // one past the item's last tile
-      const int64_t end = (last * ctas - 1) / total;
-      p.part_item[blockIdx.x] = make_int4(n, head, rtile, static_cast<int>(end - blockIdx.x));
+      record = make_int4(n, head, rtile, static_cast<int>((last * ranges - 1) / total - range));
     }
-    constexpr int CH = DB / 4;  // float4 columns of a row
-    for (int idx = tid; idx < ROWS * CH; idx += kThreads) {
-      const int row = idx / CH, c = (idx - row * CH) * 4;
-      const int r = rtile * ROWS + row;
-      if (r >= total_rows) continue;
-      const int rm = row / kRows, rr = row - rm * kRows;
-      float m = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) m = fmaxf(m, sm.m[k * MT + rm][rr]);
-      const float u = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const float f = ex2(sm.m[k * MT + rm][rr] - u);
-        const float4 x = *reinterpret_cast<const float4*>(&sm.o[k * MT + rm][rr][c]);
-        l = fmaf(sm.l[k * MT + rm][rr], f, l);
-        acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
-        acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
-      }
+    const float inv_a = complete ? row_scale(l_a) : 1.0f, inv_b = complete ? row_scale(l_b) : 1.0f;
+    const int64_t oa = static_cast<int64_t>(sl.begin + ra / p.G) * p.H_q + head * p.G + ra % p.G;
+    const int64_t ob = static_cast<int64_t>(sl.begin + rb / p.G) * p.H_q + head * p.G + rb % p.G;
+    const int64_t pa = (range * 2 + slot) * ROWS + mt * kRows + g, pb = pa + 8;
+    if (t == 0) {
       if (complete) {
-        const int64_t orow = static_cast<int64_t>(sl.begin + r / p.G) * p.H_q + head * p.G + r % p.G;
-        store_row<T>(p, orow, c, acc, m, l);
+        if (va) p.stats[oa] = row_stats(m_a, l_a);
+        if (vb) p.stats[ob] = row_stats(m_b, l_b);
       } else {
-        const int64_t prow = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * ROWS + row;
-        *reinterpret_cast<float4*>(p.part_o + prow * DB + c) = acc;
-        if (c == 0) p.part_ml[prow] = make_float2(m, l);
+        if (va) p.part_ml[pa] = make_float2(m_a, l_a);
+        if (vb) p.part_ml[pb] = make_float2(m_b, l_b);
       }
+    }
+    // Column n = 2t + e of output tile x: feature 8x + n (fp16), 32 (x / 4) + 4n + x % 4 (fp32).
+    if (HALF) {
+#pragma unroll
+      for (int x = 0; x < NO; ++x) {
+        const int col = 8 * x + 2 * t;
+        if (complete) {
+          if (col >= p.D_v) continue;
+          if (va) *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + oa * p.D_v + col) = pack_half2(o[x][0] * inv_a, o[x][1] * inv_a);
+          if (vb) *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + ob * p.D_v + col) = pack_half2(o[x][2] * inv_b, o[x][3] * inv_b);
+        } else {
+          if (va) *reinterpret_cast<float2*>(p.part_o + pa * DB + col) = make_float2(o[x][0], o[x][1]);
+          if (vb) *reinterpret_cast<float2*>(p.part_o + pb * DB + col) = make_float2(o[x][2], o[x][3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < NO; x += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = 8 * x + 4 * (2 * t + e);
+          if (complete && col >= p.D_v) continue;
+          float* const da = complete ? static_cast<float*>(p.out) + oa * p.D_v + col : p.part_o + pa * DB + col;
+          float* const db = complete ? static_cast<float*>(p.out) + ob * p.D_v + col : p.part_o + pb * DB + col;
+          if (va) store4<float>(da, o[x][e] * inv_a, o[x + 1][e] * inv_a, o[x + 2][e] * inv_a, o[x + 3][e] * inv_a);
+          if (vb) store4<float>(db, o[x][2 + e] * inv_b, o[x + 1][2 + e] * inv_b, o[x + 2][2 + e] * inv_b, o[x + 3][2 + e] * inv_b);
+        }
     }
     w += tiles;
   }
+  if (mt == 0 && lane == 0) p.part_item[range] = record;
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: a thread adds one float4 column of one row over them.
+// Joins the pieces of the item that begins in range blockIdx.x and goes on in
+// the next ones.  A thread adds one float4 column of one row over every
+// (256 / columns)-th piece; those shares are joined in shared memory.
 template <typename T, int DB, int MT>
-__global__ void __launch_bounds__(kThreads) merge_kernel(const Params p) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
   constexpr int ROWS = kRows * MT, CH = DB / 4;
+  __shared__ float4 s_acc[kMergeThreads];
+  __shared__ float2 s_ml[kMergeThreads];
   pdl_launch_dependents();
   pdl_wait();
   const int4 it = p.part_item[blockIdx.x];  // sequence, head, row tile, further pieces
   if (it.w < 0) return;
   const SeqLens sl = seq_lens(p.view, it.x);
-  const int idx = blockIdx.y * kThreads + threadIdx.x;
-  const int row = idx / CH, c = (idx - row * CH) * 4, r = it.z * ROWS + row;
-  if (r >= sl.count * p.G) return;
-  // piece 0 is slot 1 of its CTA, the others are slot 0 of theirs
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 2 + 1) * ROWS + row, step = 2 * ROWS;
-  const int64_t rest = first + ROWS;
-  float2 ml = p.part_ml[first];
-  float m = ml.x;
-  for (int i = 0; i < it.w; ++i) m = fmaxf(m, p.part_ml[rest + i * step].x);
-  const float u = m == -INFINITY ? 0.0f : m;
-  float f = ex2(ml.x - u), l = ml.y * f;
-  float4 acc = *reinterpret_cast<const float4*>(p.part_o + first * DB + c);
-  acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-#pragma unroll 4
-  for (int i = 0; i < it.w; ++i) {
-    const float2 a = p.part_ml[rest + i * step];
-    const float4 x = *reinterpret_cast<const float4*>(p.part_o + (rest + i * step) * DB + c);
-    const float w = ex2(a.x - u);
-    l = fmaf(a.y, w, l);
-    acc.x = fmaf(x.x, w, acc.x), acc.y = fmaf(x.y, w, acc.y);
-    acc.z = fmaf(x.z, w, acc.z), acc.w = fmaf(x.w, w, acc.w);
+  const int rows = min(ROWS, sl.count * p.G - it.z * ROWS);
+  const int columns = rows * CH;
+  const int at_once = min(columns, kMergeThreads);
+  const int shares = columns < kMergeThreads ? kMergeThreads / columns : 1;
+  const int share = threadIdx.x / at_once, x = threadIdx.x - share * at_once;
+  // piece 0 is slot 1 of its range, the others are slot 0 of theirs
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 2 + 1) * ROWS;
+  for (int col0 = 0; col0 < columns; col0 += kMergeThreads) {
+    const int idx = col0 + x;
+    const int row = idx / CH, c = (idx - row * CH) * 4;
+    const bool live = share < shares && idx < columns;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+#pragma unroll 8
+      for (int i = share; i <= it.w; i += shares) {
+        const int64_t piece = first + row + (i ? ROWS + static_cast<int64_t>(i - 1) * 2 * ROWS : 0);
+        const float2 ml = p.part_ml[piece];
+        join(m, l, acc, ml, *reinterpret_cast<const float4*>(p.part_o + piece * DB + c));
+      }
+    }
+    if (shares > 1) {  // (then all columns fit one round)
+      s_acc[threadIdx.x] = acc;
+      s_ml[threadIdx.x] = make_float2(m, l);
+      __syncthreads();
+      if (share == 0) {
+        for (int i = 1; i < shares; ++i) join(m, l, acc, s_ml[i * at_once + x], s_acc[i * at_once + x]);
+      }
+    }
+    if (live && share == 0) {
+      const int r = it.z * ROWS + row;
+      store_row<T>(p, static_cast<int64_t>(sl.begin + r / p.G) * p.H_q + it.y * p.G + r % p.G, c, acc, m, l);
+    }
   }
-  store_row<T>(p, static_cast<int64_t>(sl.begin + r / p.G) * p.H_q + it.y * p.G + r % p.G, c, acc, m, l);
 }
 
 }  // namespace paged

@@ -71,47 +71,25 @@ struct Piece {
   int slot;             // workspace slot (pieces > 1)
 };
 
-template <int THREADS>
-struct SchedSmem {
-  int64_t a[THREADS / 32], b[THREADS / 32];
-  Piece found;
-  int live;
-};
-
-// Inclusive prefix sum of x over the block, and its total.
-template <int THREADS>
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* warp_sums, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t v = x;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += up;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
-  }
-  return before + v;
-}
-
 __device__ __forceinline__ int pairs_of(const SeqLens& s, int tokens2) { return (s.count + tokens2 - 1) / tokens2; }
 __device__ __forceinline__ int tiles_of(const SeqLens& s) { return max(1, (s.held + kBN - 1) / kBN); }
 
-// The piece that CTA `idx` computes (from_slot: the piece in workspace slot
-// `idx`), the same for every thread; false if there is none.
-template <int THREADS>
-__device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, bool from_slot, SchedSmem<THREADS>& sm,
-                                           Piece& out) {
+__device__ __forceinline__ int64_t warp_scan(int64_t x) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, x, d);
+    if ((threadIdx.x & 31) >= d) x += up;
+  }
+  return x;
+}
+
+// The piece that CTA `idx` computes; false if there is none.  Every warp works
+// it out for itself (no barrier): lane i takes the i-th share of the sequences.
+// slots: workspace slots of the call.
+__device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, Piece& out, int& slots) {
+  const int lane = threadIdx.x & 31;
   const int tokens2 = 2 * (kBM / p.G);
-  const int per = (p.view.seqs + THREADS - 1) / THREADS, n0 = threadIdx.x * per;
-  const int n1 = min(p.view.seqs, n0 + per);
+  const int per = (p.view.seqs + 31) / 32, n0 = lane * per, n1 = min(p.view.seqs, n0 + per);
   int64_t items = 0, work = 0;
   for (int n = n0; n < n1; ++n) {
     const SeqLens s = seq_lens(p.view, n);
@@ -119,33 +97,37 @@ __device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, bool fr
     items += pr;
     work += pr * tiles_of(s);
   }
-  if (threadIdx.x == 0) sm.live = 0;
-  int64_t all_items, all_work;
-  const int64_t incl = block_scan<THREADS>(items, sm.a, all_items);
-  block_scan<THREADS>(work, sm.b, all_work);
-  all_items *= p.H_kv;
-  all_work *= p.H_kv;
+  const int64_t items_to = warp_scan(items);
+  const int64_t all_items = __shfl_sync(0xffffffffu, items_to, 31) * p.H_kv;
   const int64_t sms = p.sms;
   const bool whole = all_items >= sms;  // the first `full` items run whole
-  const int64_t rest = all_items % sms, full = whole ? all_items - rest : 0;
-  const int64_t quantum = max(static_cast<int64_t>(1), (all_work + sms - 1) / sms);
-  if (from_slot) idx += full;
-  int64_t target = idx, at = (incl - items) * p.H_kv;  // first item (piece) of this thread's sequences
+  int64_t target = idx, at = (items_to - items) * p.H_kv;  // first item (piece) of this lane's sequences
+  int64_t full = 0, quantum = 1;
   int cut = 1, piece = 0;
   if (whole) {
+    const int rest = static_cast<int>(all_items % sms);
+    full = all_items - rest;
+    const int cuts = rest ? p.sms / rest : 1;
+    slots = cuts > 1 ? rest * cuts : 0;
     if (idx >= full) {
-      cut = static_cast<int>(rest ? sms / rest : 1);
+      cut = cuts;
       target = full + (idx - full) / cut;
       piece = static_cast<int>((idx - full) % cut);
     }
   } else {
-    int64_t mine = 0, total;
+    const int64_t all_work = __shfl_sync(0xffffffffu, warp_scan(work), 31) * p.H_kv;
+    quantum = max(static_cast<int64_t>(1), (all_work + sms - 1) / sms);
+    int64_t mine = 0;
     for (int n = n0; n < n1; ++n) {
       const SeqLens s = seq_lens(p.view, n);
       mine += static_cast<int64_t>(pairs_of(s, tokens2)) * max(static_cast<int64_t>(1), tiles_of(s) / quantum);
     }
-    at = (block_scan<THREADS>(mine, sm.a, total) - mine) * p.H_kv;
+    const int64_t to = warp_scan(mine);
+    at = (to - mine) * p.H_kv;
+    slots = static_cast<int>(__shfl_sync(0xffffffffu, to, 31) * p.H_kv);
   }
+  bool found = false;
+  Piece f = {0, 0, 0, 0, 1, 0};
   for (int n = n0; n < n1; ++n) {
     const SeqLens s = seq_lens(p.view, n);
     const int64_t pr = pairs_of(s, tokens2);
@@ -157,21 +139,25 @@ __device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, bool fr
         piece = static_cast<int>(local % cut);
         local /= cut;
       }
-      Piece f;
       f.seq = n;
       f.head = static_cast<int>(local / pr);
       f.pair = static_cast<int>(pr - 1 - local % pr);  // longest causal rows first
       f.piece = piece;
       f.pieces = cut;
-      f.slot = static_cast<int>(idx - full);
-      sm.found = f;
-      sm.live = 1;
+      found = true;
     }
     at += count;
   }
-  __syncthreads();
-  out = sm.found;
-  return sm.live != 0;
+  const unsigned who = __ballot_sync(0xffffffffu, found);
+  if (!who) return false;
+  const int src = __ffs(who) - 1;
+  out.seq = __shfl_sync(0xffffffffu, f.seq, src);
+  out.head = __shfl_sync(0xffffffffu, f.head, src);
+  out.pair = __shfl_sync(0xffffffffu, f.pair, src);
+  out.piece = __shfl_sync(0xffffffffu, f.piece, src);
+  out.pieces = __shfl_sync(0xffffffffu, f.pieces, src);
+  out.slot = static_cast<int>(idx - full);
+  return true;
 }
 
 // Keys [0, lim) that token i (of the sequence's new ones) sees.
@@ -205,7 +191,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = tc::align1024(smem_raw);
   Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
-  __shared__ SchedSmem<kThreads> sched;
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x & 31;
 
@@ -225,18 +210,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     bars->abort_flag = 0;
     fence_barrier_init();
   }
-  pdl_launch_dependents();
-  pdl_wait();  // before any global access and before the wait deadline starts
-  Piece w;
-  if (!find_piece<kThreads>(p, blockIdx.x, false, sched, w)) return;  // no TMEM held yet
   if (warp == 9) tmem_alloc(&bars->tmem_base, C::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait();  // before any global access and before the wait deadline starts
   const uint32_t tmem = bars->tmem_base;
   WaitCtl ctl;
   ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;
   ctl.abort_flag = &bars->abort_flag;
+  Piece w;
+  int slots;
+  const bool live = find_piece(p, blockIdx.x, w, slots);
+  // what merge_kernel goes by: the slots, and of each slot its item (pieces in .w where it is the first of several)
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) *p.part_slots = slots;
+    if (live && w.slot >= 0 && w.slot < slots)
+      p.part_item[w.slot] = make_int4(w.seq, w.head, w.pair, w.piece == 0 && w.pieces > 1 ? w.pieces : 0);
+  }
+  if (!live) {
+    if (warp == 9) tmem_dealloc(tmem, C::kTmemCols);
+    return;
+  }
 
   const SeqLens sl = seq_lens(p.view, w.seq);
   const Range rg = range_of(p, sl, w);
@@ -539,41 +535,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of one item: grid (workspace slots, shares of its rows); a
-// thread adds one float4 column of one row over the pieces.
+// Joins the pieces of the cut items.  Units of kMergeRows rows of one slot's
+// item go round the CTAs; a thread adds one float4 column of one row over the
+// pieces.
+constexpr int kMergeRows = 32;
+constexpr int kUnits = 2 * kBM / kMergeRows;  // of a slot
+
 template <int DV>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
-  __shared__ SchedSmem<kMergeThreads> sched;
   constexpr int CH = DV / 4;
   pdl_launch_dependents();
   pdl_wait();
-  Piece w;
-  if (!find_piece<kMergeThreads>(p, blockIdx.x, true, sched, w)) return;
-  if (w.pieces == 1 || w.piece != 0) return;
-  const SeqLens sl = seq_lens(p.view, w.seq);
-  const Range rg = range_of(p, sl, w);
-  const int tpt = kBM / p.G;
-  for (int idx = blockIdx.y * kMergeThreads + threadIdx.x; idx < 2 * kBM * CH; idx += gridDim.y * kMergeThreads) {
-    const int row = idx / CH, c = (idx - row * CH) * 4;
-    const int t = row / kBM, r_in = row - t * kBM;
-    const int tok = rg.tok0 + t * tpt + r_in / p.G;
-    if (r_in >= tpt * p.G || tok >= sl.count) continue;
-    const int64_t first = static_cast<int64_t>(w.slot) * (2 * kBM) + row;
-    float m = -INFINITY;
-    for (int i = 0; i < w.pieces; ++i) m = fmaxf(m, p.part_ml[first + i * 2 * kBM].x);
-    const float u = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int units = *p.part_slots * kUnits, tpt = kBM / p.G;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int slot = unit / kUnits;
+    const int4 it = p.part_item[slot];
+    if (it.w == 0) continue;
+    const SeqLens sl = seq_lens(p.view, it.x);
+    const int tok0 = it.z * 2 * tpt;
+    for (int i = threadIdx.x; i < kMergeRows * CH; i += kMergeThreads) {
+      const int row = (unit % kUnits) * kMergeRows + i / CH, c = (i % CH) * 4;
+      const int r_in = row % kBM, tok = tok0 + row / kBM * tpt + r_in / p.G;
+      if (r_in >= tpt * p.G || tok >= sl.count) continue;
+      const int64_t first = static_cast<int64_t>(slot) * (2 * kBM) + row;
+      float m = -INFINITY, l = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = 0; i < w.pieces; ++i) {
-      const float2 a = p.part_ml[first + i * 2 * kBM];
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (first + i * 2 * kBM) * DV + c);
-      const float f = ex2(a.x - u);
-      l = fmaf(a.y, f, l);
-      acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+      for (int k = 0; k < it.w; ++k) {
+        const float2 a = p.part_ml[first + k * 2 * kBM];
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (first + k * 2 * kBM) * DV + c);
+        paged::join(m, l, acc, a, x);
+      }
+      paged::store_row<__half>(p, static_cast<int64_t>(sl.begin + tok) * p.H_q + it.y * p.G + r_in % p.G, c, acc, m, l);
     }
-    paged::store_row<__half>(p, static_cast<int64_t>(sl.begin + tok) * p.H_q + w.head * p.G + r_in % p.G, c, acc, m, l);
   }
 }
 
