@@ -22,7 +22,7 @@ int launch_t(paged::Params p, void* workspace, cudaStream_t st, int* launches) {
   const int tpt = tc::kBM / p.G;  // tokens of a row tile
   CUtensorMap mq, mk, mv;
   const int64_t page = int64_t(1) << p.view.page_shift;
-  const int box = static_cast<int>(std::min<int64_t>(page, tc::kBN));
+  const int box = static_cast<int>(std::min<int64_t>(page, paged_tc::kBN));
   if (!make_map_4d(&mq, 2, p.q, {p.D, p.G, p.H_kv, p.view.tokens}, {p.D, int64_t(p.G) * p.D, p.q_stride}, {64, p.G, 1, tpt}) ||
       !make_pool_map(&mk, 2, p.k_pages, p.view.num_pages, page, p.H_kv, p.D, box) ||
       !make_pool_map(&mv, 2, p.v_pages, p.view.num_pages, page, p.H_kv, p.D_v, box))

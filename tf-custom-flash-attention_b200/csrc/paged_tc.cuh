@@ -1,19 +1,26 @@
 // Attention of chunks of new tokens over the paged cache on the 5th-generation
 // tensor cores, fp16 in, fp32 accumulate.
 //
-// Bound: the two products (2 seen keys (D + D_v) operations a row).  The pipe
-// is the paired forward's (fwd_tc.cuh): one CTA = two 128-row tiles that share
-// every K/V tile, two softmax warpgroups alternating on the tensor pipe, one
-// TMA warp, one MMA warp.  What differs:
-//   - rows are packed (token, head of the group): a tile is floor(128 / G)
+// Bound: the two products (2 seen keys (D + D_v) operations a row) and the
+// exponentials (one a score, 16 a clock and SM).  One CTA = two 128-row tiles
+// that share every K/V tile of 64 keys: a TMA warp for K and one for V, and an
+// MMA warp and a softmax warpgroup a row tile.
+//   - Rows are packed (token, head of the group): a tile is floor(128 / G)
 //     tokens x G heads, so the G heads of a KV head share one reading of it;
-//     Q comes as one box (64 columns, G heads, 1 KV head, tokens) a tile;
-//   - a K/V tile of 128 keys is 128 / min(page, 128) boxes, one page each, one
-//     issued by each lane of the TMA warp (a page's boxes need its table entry
-//     first; the entries of the next tile are read a tile ahead);
-//   - keys behind the sequence are masked, and their V rows set to zero in
-//     shared memory before the product (0 * NaN is NaN);
-//   - long sequences with few rows are cut along the keys (below).
+//     Q comes as one box (64 columns, G heads, 1 KV head, tokens) a tile.
+//   - A K/V tile is 64 / min(page, 64) boxes, one page each, one issued by each
+//     lane of the TMA warp (a page's boxes need its table entry first; the
+//     entries of the next tile are read a tile ahead).
+//   - Two score buffers a row tile: S(i+1) is there when the softmax of tile i
+//     ends, and PV(i), S(i+2) are issued while it works on i+1, so neither the
+//     products nor the barriers between the warps (~300 cycles from an arrival
+//     to the waiter) stand in its way.  TMEM, 512 columns: O 2 x 128, and for
+//     each row tile two slots of 64 columns, where P (fp16, 32 columns) goes
+//     over S.  With tiles of 128 keys there is room for one slot a row tile:
+//     softmax (1900 cycles) and products (2100 with their waits) took turns,
+//     4000 cycles a tile of 128 keys for D = 128 and for D = 64.
+//   - Keys behind the sequence are masked, and their V rows set to zero in
+//     shared memory before the product (0 * NaN is NaN).
 //
 // Work: an item is a pair of row tiles of one (sequence, KV head).  With at
 // least as many items as SMs they run whole, but for the last items % SMs,
@@ -30,39 +37,125 @@ namespace paged_tc {
 
 using paged::Params;
 using tc::kBM;
-using tc::kBN;
 using tc::warp_wait;
 
-constexpr int kThreads = 320;
+constexpr int kBN = 64;  // keys of a tile
+
+constexpr int kThreads = 384;  // warps 0-7 softmax, 8 Q and K, 9 and 10 MMA, 11 V
+
+// The MMA warps stay converged: every lane runs the loop and one elected lane
+// issues, by a predicate on the instruction.  In a branch of one lane the
+// compiler has to move every operand to the uniform registers that tcgen05
+// takes: 870 cycles to issue eight MMAs, where their work is 256 (D = 64).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(one)
+      : "memory");
+}
 constexpr int kMergeThreads = 256;
 
 template <int DQK, int DV>
 struct Cfg {
-  static constexpr int kStages = (DQK + DV > 128) ? 2 : 4;
-  static constexpr uint32_t kQBytes = kBM * DQK * 2;  // one tile
+  static constexpr int kStages = 5;  // of the K ring and of the V ring
+  static constexpr uint32_t kQBytes = kBM * DQK * 2;  // one row tile
   static constexpr uint32_t kKBytes = kBN * DQK * 2;
   static constexpr uint32_t kVBytes = kBN * DV * 2;
   static constexpr uint32_t kKOff = 2 * kQBytes;
   static constexpr uint32_t kVOff = kKOff + kStages * kKBytes;
   static constexpr uint32_t kBarOff = kVOff + kStages * kVBytes;
-  static constexpr uint32_t kSmemBytes = kBarOff + 256 + 1024;
+  static constexpr uint32_t kSmemBytes = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kTmemCols = 512;
-  static_assert(256 + 2 * DV <= 512, "TMEM budget");
+  static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 };
 
 struct Barriers {
   uint64_t q_full;
-  uint64_t k_full[4];
-  uint64_t v_full[4];
-  uint64_t kv_empty[4];
-  uint64_t s_full[2];  // per row tile
-  uint64_t p_full[2];
-  uint64_t o_done[2];
-  uint64_t mma_done;
+  uint64_t k_full[5], k_empty[5];
+  uint64_t v_full[5], v_empty[5];
+  uint64_t s_full[2][2];  // row tile, slot
+  uint64_t p_full[2][2];
+  uint64_t o_done[2];     // every PV of the row tile
+  uint64_t o_final[2];    // its last
+  uint64_t mma_done[2];
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Barriers) <= 256, "barrier space");
+static_assert(sizeof(Barriers) <= 512, "barrier space");
+
+constexpr int kPolyOf8 = 2;  // of 8 pairs of scores, those whose exponentials go to the FMA pipe
+// 2^(r s + b) for two scores on the FMA pipe, for a part of the exponentials,
+// to relieve the special function unit: x = n + f with n the nearest integer
+// (by the addition of 1.5 * 2^23), |f| <= 1/2, 2^f by a polynomial of degree 4
+// (least squares at Chebyshev nodes; off by 4e-6 at most, a sixtieth of the
+// rounding of P to fp16), n added to the exponent.  x below -126 gives 2^-126,
+// which fp16 rounds to zero.
+__device__ __forceinline__ void exp2_pair(float& p0, float& p1, float r0, float r1, float s, float b) {
+  float x0, x1, n0, n1, f0, f1;
+  ffma2(x0, x1, r0, r1, s, s, b, b);
+  x0 = fmaxf(x0, -126.0f), x1 = fmaxf(x1, -126.0f);
+  constexpr float kMagic = 12582912.0f;
+  n0 = kMagic, n1 = kMagic;
+  fadd2(n0, n1, x0, x1);
+  float m0 = -kMagic, m1 = -kMagic;
+  fadd2(m0, m1, n0, n1);                                   // n
+  ffma2(f0, f1, m0, m1, -1.0f, -1.0f, x0, x1);             // f
+  ffma2(p0, p1, f0, f1, 0.00957010128f, 0.00957010128f, 0.0559178591f, 0.0559178591f);
+  ffma2(p0, p1, p0, p1, f0, f1, 0.240247443f, 0.240247443f);
+  ffma2(p0, p1, p0, p1, f0, f1, 0.693121791f, 0.693121791f);
+  ffma2(p0, p1, p0, p1, f0, f1, 0.999999285f, 0.999999285f);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
+
+// Whether three barriers have all passed (one vote: 75 cycles; three waits one
+// after the other, each for a phase long over, take 280).
+__device__ __forceinline__ bool test3(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, uint64_t* c, uint32_t pc) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "and.pred p, p, q;\n\tand.pred p, p, r;\n\t"
+      "vote.sync.all.pred p, p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(a)), "r"(pa), "r"(smem_u32(b)), "r"(pb), "r"(smem_u32(c)), "r"(pc)
+      : "memory");
+  return ok != 0;
+}
 
 // ---------------------------------------------------------------- the cut
 struct Piece {
@@ -198,15 +291,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars->q_full, 1);
     for (int s = 0; s < ST; ++s) {
       mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 2);  // both MMA warps
       mbar_init(&bars->v_full[s], 1);
-      mbar_init(&bars->kv_empty[s], 1);
+      mbar_init(&bars->v_empty[s], 2);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], kBM);
-      mbar_init(&bars->o_done[s], 1);
+    for (int t = 0; t < 2; ++t) {
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&bars->s_full[t][s], 1);
+        mbar_init(&bars->p_full[t][s], kBM);
+      }
+      mbar_init(&bars->o_done[t], 1);
+      mbar_init(&bars->o_final[t], 1);
+      mbar_init(&bars->mma_done[t], 1);
     }
-    mbar_init(&bars->mma_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
   }
@@ -246,56 +343,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     n_t[1] = rg.tok0 + tpt < sl.count ? n_kv : 0;
   }
 
-  if (warp == 8) {
-    // ------------------------------------------------------ TMA producer
+  if (warp == 8 || warp == 11) {
+    // ------------------------------------- TMA: K (and Q) by warp 8, V by warp 11
     if (n_kv > 0) {
+      const bool is_k = warp == 8;
       const int box = min(kBN, 1 << p.view.page_shift);
-      const int subs = kBN / box;                         // boxes of a column block
-      constexpr int KC = DQK / 64, VC = DV / 64;
-      const int loads = subs * (KC + VC);                 // a tile's, at most 8 * 4 = 32
-      const int sub = lane % subs, chunk = lane / subs;   // this lane's
-      const bool mine = lane < loads, is_k = chunk < KC;
+      const int subs = kBN / box;                    // boxes of a column block
+      const int chunks = is_k ? DQK / 64 : DV / 64;  // column blocks
+      const int sub = lane % subs, chunk = lane / subs;  // this lane's box (at most 4 x 2)
+      const bool mine = chunk < chunks;
       const int page_mask = (1 << p.view.page_shift) - 1;
+      const CUtensorMap* const map = is_k ? &tm_k : &tm_v;
+      uint64_t* const full = is_k ? bars->k_full : bars->v_full;
+      uint64_t* const empty = is_k ? bars->k_empty : bars->v_empty;
+      const uint32_t stage_bytes = is_k ? C::kKBytes : C::kVBytes;
+      uint8_t* const dst0 = smem + (is_k ? C::kKOff : C::kVOff) + chunk * kBN * 128 + sub * box * 128;
       if (lane == 0) {
-        tma_prefetch_desc(&tm_q);
-        tma_prefetch_desc(&tm_k);
-        tma_prefetch_desc(&tm_v);
-        // boxes of tpt tokens x G heads: tpt * G rows of each tile
-        mbar_expect_tx(&bars->q_full, 2u * static_cast<uint32_t>(KC * tpt * p.G * 128));
+        tma_prefetch_desc(map);
+        if (is_k) {
+          tma_prefetch_desc(&tm_q);
+          // boxes of tpt tokens x G heads: tpt * G rows of each tile
+          mbar_expect_tx(&bars->q_full, 2u * static_cast<uint32_t>(DQK / 64 * tpt * p.G * 128));
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int c = 0; c < KC; ++c)
-            tma_load_4d(smem + t * C::kQBytes + c * kBM * 128, &tm_q, c * 64, 0, w.head, sl.begin + rg.tok0 + t * tpt,
-                        &bars->q_full);
+            for (int c = 0; c < DQK / 64; ++c)
+              tma_load_4d(smem + t * C::kQBytes + c * kBM * 128, &tm_q, c * 64, 0, w.head, sl.begin + rg.tok0 + t * tpt,
+                          &bars->q_full);
+        }
       }
       auto page_at = [&](int j) {
         const int key = (rg.j0 + j) * kBN + sub * box;
-        return mine && j < n_kv && key < sl.held ? page_of(p.view, w.seq, key >> p.view.page_shift) : -2;
+        return mine && j < n_kv && key < sl.held ? page_of(p.view, w.seq, key >> p.view.page_shift) : -1;
       };
-      int page = page_at(0), issued = 0;
+      int page = page_at(0), issued = 0, s = 0;
+      uint32_t phase = 1;
       for (int j = 0; j < n_kv; ++j) {
-        const int s = j % ST;
         const int next = page_at(j + 1);
-        if (!warp_wait(&bars->kv_empty[s], ((j / ST) & 1) ^ 1, ctl)) break;
         const int key0 = (rg.j0 + j) * kBN;
         const int boxes = min(subs, (sl.held - key0 + box - 1) / box);  // boxes that hold keys of the sequence
-        if (lane == 0) {
-          mbar_expect_tx(&bars->k_full[s], static_cast<uint32_t>(KC * boxes * box * 128));
-          mbar_expect_tx(&bars->v_full[s], static_cast<uint32_t>(VC * boxes * box * 128));
-        }
+        if (!warp_wait(&empty[s], phase, ctl)) break;
+        if (lane == 0) mbar_expect_tx(&full[s], static_cast<uint32_t>(chunks * boxes * box * 128));
         __syncwarp();
-        if (mine && sub < boxes) {  // a page id outside the pool (-1) reads as zeros
-          const int row = (key0 + sub * box) & page_mask;
-          if (is_k)
-            tma_load_4d(smem + C::kKOff + s * C::kKBytes + chunk * kBN * 128 + sub * box * 128, &tm_k, chunk * 64, w.head,
-                        row, page, &bars->k_full[s]);
-          else
-            tma_load_4d(smem + C::kVOff + s * C::kVBytes + (chunk - KC) * kBN * 128 + sub * box * 128, &tm_v,
-                        (chunk - KC) * 64, w.head, row, page, &bars->v_full[s]);
-        }
+        if (mine && sub < boxes)  // a page id outside the pool (-1) reads as zeros
+          tma_load_4d(dst0 + s * stage_bytes, map, chunk * 64, w.head, (key0 + sub * box) & page_mask, page, &full[s]);
         issued = j + 1;
         page = next;
+        if (++s == ST) s = 0, phase ^= 1;
       }
       __syncwarp();
       if (*ctl.abort_flag && lane == 0) {  // let copies in flight land before the CTA exits
@@ -303,67 +397,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         drain.deadline_ns = globaltimer_ns() + p.timeout_ns;
         int dummy = 0;
         drain.abort_flag = &dummy;
-        mbar_wait(&bars->q_full, 0, drain);
-        for (int j = (issued > ST ? issued - ST : 0); j < issued; ++j) {
-          mbar_wait(&bars->k_full[j % ST], (j / ST) & 1, drain);
-          mbar_wait(&bars->v_full[j % ST], (j / ST) & 1, drain);
-        }
+        if (is_k) mbar_wait(&bars->q_full, 0, drain);
+        for (int j = max(0, issued - ST); j < issued; ++j) mbar_wait(&full[j % ST], (j / ST) & 1, drain);
       }
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------- MMA issuer
-    if (lane == 0 && n_kv > 0) {
+  } else if (warp == 9 || warp == 10) {
+    // ------------------------------------------- MMA issuer of row tile t
+    if (n_kv > 0) {
       constexpr uint32_t idesc_qk = make_idesc(kBM, kBN, false, false, false);
       constexpr uint32_t idesc_pv = make_idesc(kBM, DV, false, true, false);
-      const uint32_t sQ = smem_u32(smem);
-      const uint32_t sK0 = smem_u32(smem + C::kKOff);
-      const uint32_t sV0 = smem_u32(smem + C::kVOff);
-      auto issue_s = [&](int t, int j) -> bool {  // S_t = Q_t K_j^T
-        const int s = j % ST;
-        if (!mbar_wait(&bars->k_full[s], (j / ST) & 1, ctl)) return false;
-        tc_fence_after();
-        const uint32_t kbase = sK0 + s * C::kKBytes, qbase = sQ + t * C::kQBytes;
+      const int t = warp - 9, n_my = t ? n_t[1] : n_t[0];
+      const uint32_t one = elect_one();
+      // descriptors of stage 0; an offset of n bytes adds n / 16
+      const uint64_t q_desc = make_sw128_desc(smem_u32(smem + t * C::kQBytes), 16, 1024);
+      const uint64_t k_desc = make_sw128_desc(smem_u32(smem + C::kKOff), 16, 1024);
+      const uint64_t v_desc = make_sw128_desc(smem_u32(smem + C::kVOff), kBN * 128, 1024);
+      const uint32_t tO = tmem + t * 128, tS = tmem + 256 + t * 128;
+      int ks = 0, vs = 0;  // stage of the next K and V tile, and their phases
+      uint32_t kph = 0, vph = 0;
+      auto issue_s = [&](int j) {  // S(j) = Q K_j^T, to slot j % 2; K_j is there
+        if (j < n_my) {
 #pragma unroll
-        for (int kk = 0; kk < DQK / 16; ++kk) {
-          const uint32_t koff = (kk >> 2) * (kBM * 128) + (kk & 3) * 32;
-          mma_f16_ss(tmem + t * 128, make_sw128_desc(qbase + koff, 16, 1024), make_sw128_desc(kbase + koff, 16, 1024),
-                     idesc_qk, kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < DQK / 16; ++kk) {
+            const uint32_t in = (kk & 3) * 32;
+            mma_ss(one, tS + (j & 1) * kBN, q_desc + ((kk >> 2) * (kBM * 128) + in) / 16,
+                   k_desc + (ks * C::kKBytes + (kk >> 2) * (kBN * 128) + in) / 16, idesc_qk, kk > 0 ? 1u : 0u);
+          }
+          commit(one, &bars->s_full[t][j & 1]);
         }
-        mma_commit(&bars->s_full[t]);
-        return true;
+        commit(one, &bars->k_empty[ks]);  // (an arrival alone where this row tile does not need the tile)
+        if (++ks == ST) ks = 0, kph ^= 1;
       };
-      auto issue_pv = [&](int t, int j) -> bool {  // O_t += P_t V_j
-        const int s = j % ST;
-        if (!mbar_wait(&bars->p_full[t], j & 1, ctl)) return false;
-        if (!mbar_wait(&bars->v_full[s], (j / ST) & 1, ctl)) return false;
+      bool ok = warp_wait(&bars->q_full, 0, ctl);
+      for (int j = 0; ok && j < min(2, n_kv); ++j) {
+        ok = warp_wait(&bars->k_full[ks], kph, ctl);
         tc_fence_after();
-        const uint32_t vbase = sV0 + s * C::kVBytes;
-#pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          mma_f16_ts(tmem + 256 + t * DV, tmem + t * 128 + kk * 8,
-                     make_sw128_desc(vbase + kk * 16 * 128, kBN * 128, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-        mma_commit(&bars->o_done[t]);
-        return true;
-      };
-      bool ok = mbar_wait(&bars->q_full, 0, ctl);
-      if (ok && n_t[0] > 0) ok = issue_s(0, 0);
-      if (ok && n_t[1] > 0) ok = issue_s(1, 0);
-      for (int j = 0; ok && j < n_kv; ++j) {
-        if (j < n_t[0]) {
-          ok = issue_pv(0, j);
-          if (ok && j + 1 < n_t[0]) ok = issue_s(0, j + 1);
-        }
-        if (ok && j < n_t[1]) ok = issue_pv(1, j);
-        if (!ok) break;
-        mma_commit(&bars->kv_empty[j % ST]);  // K_j, V_j no longer read
-        if (j + 1 < n_t[1]) ok = issue_s(1, j + 1);
+        if (ok) issue_s(j);
       }
-      mma_commit(&bars->mma_done);  // every MMA issued so far must finish before TMEM is released
+      for (int j = 0; ok && j < n_kv; ++j) {
+        // V_j, K_{j+2} (where there is one) and P(j) (where this row tile needs V_j)
+        uint64_t* const vb = &bars->v_full[vs];
+        uint64_t* const kb = j + 2 < n_kv ? &bars->k_full[ks] : vb;
+        uint64_t* const pb = j < n_my ? &bars->p_full[t][j & 1] : vb;
+        const uint32_t kp = j + 2 < n_kv ? kph : vph, pp = j < n_my ? (j >> 1) & 1 : vph;
+        if (!test3(vb, vph, kb, kp, pb, pp) &&
+            (!warp_wait(vb, vph, ctl) || !warp_wait(kb, kp, ctl) || !warp_wait(pb, pp, ctl))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (j < n_my) {
+#pragma unroll
+          for (int kk = 0; kk < kBN / 16; ++kk)  // O += P(j) V_j
+            mma_ts(one, tO, tS + (j & 1) * kBN + kk * 8, v_desc + (vs * C::kVBytes + kk * 16 * 128) / 16, idesc_pv,
+                   (j > 0 || kk > 0) ? 1u : 0u);
+          commit(one, &bars->o_done[t]);
+          if (j == n_my - 1) commit(one, &bars->o_final[t]);
+        }
+        commit(one, &bars->v_empty[vs]);
+        if (++vs == ST) vs = 0, vph ^= 1;
+        if (j + 2 < n_kv) issue_s(j + 2);
+      }
+      commit(one, &bars->mma_done[t]);  // every MMA issued so far must finish before TMEM is released
       WaitCtl drain = ctl;
       drain.deadline_ns = globaltimer_ns() + p.timeout_ns;
       int dummy = 0;
       drain.abort_flag = &dummy;
-      mbar_wait(&bars->mma_done, 0, drain);
+      if (lane == 0) mbar_wait(&bars->mma_done[t], 0, drain);
     }
   } else {
     // ------------------------------------------------ softmax warpgroups
@@ -371,8 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wq = warp & 3;          // TMEM lane quadrant
     const int r_in = wq * 32 + lane;  // TMEM lane = packed row of the tile
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t tS = tmem + lane_base + t * 128;
-    const uint32_t tO = tmem + lane_base + 256 + t * DV;
+    const uint32_t tO = tmem + lane_base + t * 128;
     const int tok = rg.tok0 + t * tpt + r_in / p.G;  // of the sequence's new tokens
     const bool active = r_in < tpt * p.G && tok < sl.count;
     const bool warp_active = __any_sync(0xffffffffu, active);
@@ -386,100 +485,105 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m_use = -INFINITY;  // reference max the exponentials are taken against
     float l = 0.0f;           // sum of exp2(x - m_use)
     bool ok = true;
-    for (int j = 0; j < n_my; ++j) {
-      if (!warp_wait(&bars->s_full[t], j & 1, ctl)) {
-        ok = false;
-        break;
-      }
+    const uint32_t tS0 = tmem + lane_base + 256 + t * 128;
+    auto step = [&](int j) -> bool {  // softmax of tile j
+      uint32_t r[kBN];
+      if (!warp_wait(&bars->s_full[t][j & 1], (j >> 1) & 1, ctl)) return false;
       tc_fence_after();
-      const int kv0 = (rg.j0 + j) * kBN;
-      if (kv0 + kBN > sl.held && (t == 0 || j >= n_t[0])) {
-        // the first user of V_j clears its rows behind the sequence (thread r: row r)
-        const int s = j % ST;
-        if (!warp_wait(&bars->v_full[s], (j / ST) & 1, ctl)) {
-          ok = false;
-          break;
-        }
-        if (kv0 + r_in >= sl.held) {
+      SDPA_TMEM_LD32(tS0 + (j & 1) * kBN, (r + 0));
+      SDPA_TMEM_LD32(tS0 + (j & 1) * kBN + 32, (r + 32));
+      tmem_wait_ld();
+      if ((rg.j0 + j + 1) * kBN > lim_w || !fold) {  // some row does not see the whole tile, or a scale <= 0
+        const int left = max(0, min(kBN, lim - (rg.j0 + j) * kBN));
 #pragma unroll
-          for (int c = 0; c < DV / 64; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(smem + C::kVOff + s * C::kVBytes + c * kBN * 128 + r_in * 128);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
-          }
+        for (int c = 0; c < kBN; ++c) {
+          const float x = __uint_as_float(r[c]);
+          r[c] = __float_as_uint(c >= left ? -INFINITY : fold ? x : x * p.scale_log2);
         }
-        fence_proxy_async_smem();
       }
-      if (warp_active) {
-        uint32_t r[128];
-        SDPA_TMEM_LD32(tS + 0, (r + 0));
-        SDPA_TMEM_LD32(tS + 32, (r + 32));
-        SDPA_TMEM_LD32(tS + 64, (r + 64));
-        SDPA_TMEM_LD32(tS + 96, (r + 96));
-        tmem_wait_ld();
-        if (!fold) {
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four independent chains
 #pragma unroll
-          for (int c = 0; c < 128; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * p.scale_log2);
-        }
-        if (kv0 + kBN > lim_w) {  // some row of the warp does not see the whole tile
-          const int left = max(0, min(kBN, lim - kv0));
+      for (int c = 0; c < kBN; c += 8)
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= left) r[c] = __float_as_uint(-INFINITY);
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four independent chains
-#pragma unroll
-        for (int c = 0; c < 128; c += 8)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mx[q] = fmax3(mx[q], __uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
-        const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scl;
-        m_run = fmaxf(m_run, tmax);
-        float alpha = 1.0f;
-        bool rescale_o = false;
-        if (tmax > m_use + tc::kRescaleThreshold) {
-          alpha = ex2(m_use - m_run);  // 0 when m_use = -inf
-          rescale_o = (j > 0) && (m_use != -INFINITY);
-          m_use = m_run;
-          l *= alpha;
-        }
-        const float nmu = (m_use == -INFINITY) ? 0.0f : -m_use;
-        float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(r[c]), scl, nmu));
-          const float p1 = ex2(fmaf(__uint_as_float(r[c + 1]), scl, nmu));
-          rs[(c >> 1) & 3] += p0 + p1;
-          r[c / 2] = pack_half2(p0, p1);  // p <= 2^8 enters the product as fp16; the sum l keeps fp32
-        }
-        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-        SDPA_TMEM_ST32(tS + 0, (r + 0));
-        SDPA_TMEM_ST32(tS + 32, (r + 32));
-        if (__any_sync(0xffffffffu, rescale_o)) {
-          // O_t holds PV_t(j-1) (committed before S_t(j)); rescale it before PV_t(j)
-          if (!warp_wait(&bars->o_done[t], (j - 1) & 1, ctl)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const float a = rescale_o ? alpha : 1.0f;
-#pragma unroll
-          for (int c = 0; c < DV / 32; ++c) {
-            uint32_t o[32];
-            SDPA_TMEM_LD32(tO + c * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-            SDPA_TMEM_ST32(tO + c * 32, o);
-          }
-        }
-        tmem_wait_st();
+        for (int q = 0; q < 4; ++q)
+          mx[q] = fmax3(mx[q], __uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
+      const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scl;
+      m_run = fmaxf(m_run, tmax);
+      float alpha = 1.0f;
+      bool rescale_o = false;
+      if (tmax > m_use + tc::kRescaleThreshold) {
+        alpha = ex2(m_use - m_run);  // 0 when m_use = -inf
+        rescale_o = (j > 0) && (m_use != -INFINITY);
+        m_use = m_run;
+        l *= alpha;
       }
+      const float nmu = (m_use == -INFINITY) ? 0.0f : -m_use;
+      float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < kBN; c += 2) {
+        float p0, p1;
+        if (c / 2 % 8 < kPolyOf8) {
+          exp2_pair(p0, p1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), scl, nmu);
+        } else {
+          p0 = ex2(fmaf(__uint_as_float(r[c]), scl, nmu));
+          p1 = ex2(fmaf(__uint_as_float(r[c + 1]), scl, nmu));
+        }
+        rs[(c >> 1) & 3] += p0 + p1;
+        r[c / 2] = pack_half2(p0, p1);  // p <= 2^8 enters the product as fp16; the sum l keeps fp32
+      }
+      l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      SDPA_TMEM_ST32(tS0 + (j & 1) * kBN, r);
+      if (__any_sync(0xffffffffu, rescale_o)) {
+        // PV(j-1) must have finished (it may still run), PV(j) waits for this warp
+        if (!warp_wait(&bars->o_done[t], (j - 1) & 1, ctl)) return false;
+        tc_fence_after();
+        const float a = rescale_o ? alpha : 1.0f;
+#pragma unroll
+        for (int c = 0; c < DV / 32; ++c) {
+          uint32_t o[32];
+          SDPA_TMEM_LD32(tO + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+          SDPA_TMEM_ST32(tO + c * 32, o);
+        }
+      }
+      tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&bars->p_full[t]);
+      mbar_arrive(&bars->p_full[t][j & 1]);
+      return true;
+    };
+    // V_j's rows behind the sequence are cleared before its product (thread r: row r; by both row tiles, whose
+    // products are not ordered)
+    auto clear_v = [&](int j) -> bool {
+      const int s = j % ST;
+      if (!warp_wait(&bars->v_full[s], (j / ST) & 1, ctl)) return false;
+      if (r_in < kBN && (rg.j0 + j) * kBN + r_in >= sl.held) {
+#pragma unroll
+        for (int c = 0; c < DV / 64; ++c) {
+          uint4* row = reinterpret_cast<uint4*>(smem + C::kVOff + s * C::kVBytes + c * kBN * 128 + r_in * 128);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+      return true;
+    };
+    const int j_clear = n_my > 0 && (rg.j0 + n_my) * kBN > sl.held ? n_my - 1 : -1;  // the tile that holds the last key
+    if (warp_active) {
+      for (int j = 0; ok && j < n_my; ++j) {
+        if (j == j_clear) ok = clear_v(j);
+        if (ok) ok = step(j);
+      }
+    } else {  // no row of this warp has a token: it only keeps the barriers' counts
+      for (int j = 0; ok && j < n_my; ++j) {
+        if (j == j_clear) ok = clear_v(j);
+        if (ok) ok = warp_wait(&bars->s_full[t][j & 1], (j >> 1) & 1, ctl);
+        if (ok) mbar_arrive(&bars->p_full[t][j & 1]);
+      }
     }
     // ----------------------------------------------------------- epilogue
-    if (ok && n_my > 0) ok = warp_wait(&bars->o_done[t], (n_my - 1) & 1, ctl);
+    if (ok && n_my > 0) ok = warp_wait(&bars->o_final[t], 0, ctl);
     if (ok && warp_active) {
       tc_fence_after();
       const float f = m_run == -INFINITY ? 0.0f : ex2(m_use - m_run);
