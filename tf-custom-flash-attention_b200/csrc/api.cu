@@ -576,12 +576,13 @@ int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void*
   t_launches = 0;
   if (!serving_shape(dtype, D) || !serving_shape(dtype, D_v)) return SDPA_B200_EINVAL;
   if (D > 128 || D_v > 128) return SDPA_B200_EUNSUPPORTED;
-  if (H_kv < 1 || H_q < H_kv || H_q % H_kv != 0) return SDPA_B200_EINVAL;
+  if (H_kv < 1 || H_q < H_kv || H_q % H_kv != 0 || H_kv > 32767) return SDPA_B200_EINVAL;
   paged::Params p;
   std::memset(&p, 0, sizeof(p));
   if (int e = fill_view(p.view, page_table, table_width, kv_len, q_start, seqs, num_pages, page_size, tokens)) return e;
   if (tokens == 0 || seqs == 0) return SDPA_B200_OK;
-  if (H_q > kIntMax / tokens) return SDPA_B200_EINVAL;  // packed rows are counted in 32 bits
+  // packed rows and items of work are counted in 32 bits
+  if (H_q > kIntMax / 4 / tokens || H_kv > kIntMax / 4 / seqs) return SDPA_B200_EINVAL;
   if (!q || !out || !stats || !aligned16(q) || !aligned16(out) || !stride_ok(dtype, q_stride, H_q * D)) return SDPA_B200_EINVAL;
   if (num_pages < 1 || !k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages)) return SDPA_B200_EINVAL;
   if (!workspace || !aligned16(workspace) ||

@@ -226,8 +226,8 @@ int launch_rotary_fwd(int dtype, const rotary::Params& p, cudaStream_t st, int* 
 int launch_rotary_bwd(int dtype, const rotary::Params& p, cudaStream_t st, int* launches);
 int launch_paged_append(int dtype, const rotary::Params& p, cudaStream_t st, int* launches);
 int launch_paged_sdpa(int dtype, paged::Params p, void* workspace, cudaStream_t st, int* launches);
-int launch_paged_tc(const paged::Params& p, void* workspace, cudaStream_t st, int* launches);
-size_t paged_tc_workspace_bytes(int D_v);
+int launch_paged_tc(const paged::Params& p, cudaStream_t st, int* launches);
+size_t place_paged_tc(paged::Params* p, void* w, int D_v);
 size_t paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v);
 // Reads and clears the status word of each translation unit's kernels.
 int status_exchange_fwd_tc(unsigned int* w);

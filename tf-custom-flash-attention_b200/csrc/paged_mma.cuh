@@ -1,5 +1,5 @@
 // Attention of new tokens over the paged cache, for sequences with few of
-// them (single tokens, drafted ones), fp16 and fp32.
+// them (single tokens, drafted ones) in fp16, and for all in fp32.
 //
 //   o_i = sum_j softmax_j(scale q_i.k_j) v_j,   stats_i = max + ln(sum + 1e-6)
 //
@@ -51,11 +51,17 @@ struct Params {
   int H_q, H_kv, G, D, D_v;
   float scale_log2;
   int causal;
-  // workspace
-  float* part_o;          // [ranges, 2, rows, DB] unnormalised sums
-  float2* part_ml;        // [ranges, 2, rows] (max, sum), log2 units
-  int4* part_item;        // [ranges] (sequence, head, row tile, ranges after this one that hold the rest; -1: none)
-  int* part_slots;        // tcgen05 kernel: slots of the call (its part_item: [slots] items)
+  // workspace of the kernel for few rows: items cut between ranges
+  float* part_o;          // [ranges, 2, part_rows, part_cols] unnormalised sums
+  float2* part_ml;        // [ranges, 2, part_rows] (max, sum), log2 units
+  int4* part_item;        // [ranges] of the item cut at the range's end: (its sequence's first token, its first
+                          // packed row, its rows, KV head << 16 | ranges behind that hold the rest); 0 rows: none
+  int part_ranges, part_rows, part_cols;
+  // workspace of the chunk kernel: pieces of cut items
+  float* tc_o;            // [slots, 256, DV]
+  float2* tc_ml;          // [slots, 256]
+  int4* tc_item;          // [slots] (the pair's first token, its tokens, KV head, pieces << 16 | this one's index)
+  int* tc_slots;          // slots in use
   int sms;                // SMs of the device
   uint64_t timeout_ns;
 };
@@ -191,7 +197,6 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   pdl_launch_dependents();
   pdl_wait();
   WaitCtl ctl;
-  ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;
   ctl.abort_flag = &s_abort;
 
   // ---- this group's range of tiles
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   const int64_t range = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(gridDim.x) * group;
   const int64_t ranges = min(static_cast<int64_t>(gridDim.x) * S::kGroups, total);
   if (range >= ranges) {
-    if (mt == 0 && lane == 0) p.part_item[range] = make_int4(0, 0, 0, -1);
+    if (mt == 0 && lane == 0) p.part_item[range] = make_int4(0, 0, 0, 0);
     return;
   }
   const int64_t w0 = total * range / ranges, w1 = total * (range + 1) / ranges;
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   for (int i = 0; i < kWarps; ++i) c += __popc(__ballot_sync(0xffffffffu, s_before[i * 32 + lane] <= w0));
   int n = (c - 1) * per;
   int64_t base = s_before[c - 1];
-  int4 record = make_int4(0, 0, 0, -1);
+  int4 record = make_int4(0, 0, 0, 0);
 
   const int page_shift = p.view.page_shift, page_mask = (1 << page_shift) - 1;
   // this lane's row and 16-byte chunk in the ldmatrix loads of K and V (chunk ^ row % 8: the swizzle)
@@ -252,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
       ++n;
       continue;
     }
+    ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;  // (of each item)
     const int64_t local = w - base;
     const int64_t item = local / nt;
     const int tile0 = static_cast<int>(local - item * nt);
@@ -493,7 +499,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     const int slot = tile0 == 0 ? 1 : 0;  // 0: the item began before this range
     if (!complete && slot == 1) {
       const int64_t last = base + (item + 1) * nt;  // one past the item's last tile
-      record = make_int4(n, head, rtile, static_cast<int>((last * ranges - 1) / total - range));
+      record = make_int4(sl.begin, rtile * ROWS, min(ROWS, total_rows - rtile * ROWS),
+                         head << 16 | static_cast<int>((last * ranges - 1) / total - range));
     }
     const float inv_a = complete ? row_scale(l_a) : 1.0f, inv_b = complete ? row_scale(l_b) : 1.0f;
     const int64_t oa = static_cast<int64_t>(sl.begin + ra / p.G) * p.H_q + head * p.G + ra % p.G;
@@ -540,52 +547,85 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   if (mt == 0 && lane == 0) p.part_item[range] = record;
 }
 
-// Joins the pieces of the item that begins in range blockIdx.x and goes on in
-// the next ones.  A thread adds one float4 column of one row over every
-// (256 / columns)-th piece; those shares are joined in shared memory.
-template <typename T, int DB, int MT>
+// Joins the pieces of cut items (the item that begins in range i and goes on in
+// the next ones), which go round the blocks in turn.  A thread adds float4
+// columns of a row over the pieces, whose values it reads several at a time
+// (latency bounds this kernel); for items of few rows over every (shares)-th
+// piece, the shares joined in shared memory.
+
+// Pieces at rows first, first + step, .. (count of them) of one float4 column.
+// All offsets fit 32 bits (the workspace is some tens of MB).
+template <int AHEAD>
+__device__ __forceinline__ void join_pieces(const float* o, const float2* ml, int first, int step, int count, int cols,
+                                            float& m, float& l, float4& acc) {
+  for (; count > 0; count -= AHEAD, first += AHEAD * step) {
+    float2 a[AHEAD];
+    float4 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < count) {
+        a[i] = ml[first + i * step];
+        x[i] = *reinterpret_cast<const float4*>(o + (first + i * step) * cols);
+      }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < count) join(m, l, acc, a[i], x[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void merge_range(const Params& p, int range, const int4& it, float4* s_acc, float2* s_ml) {
+  const int ROWS = p.part_rows, shift = p.part_cols == 64 ? 4 : 5;  // log2 of a row's float4 columns
+  const int rows = it.z, pieces = (it.w & 0xffff) + 1, head = it.w >> 16;
+  // rows a round takes, and (where the item has fewer) shares of the pieces
+  const int round = kMergeThreads >> shift, at_once = min(rows, round), shares = min(pieces, round / at_once);
+  const int group = threadIdx.x >> shift, c = (threadIdx.x & ((1 << shift) - 1)) * 4;
+  const int share = group / at_once, row_in = group - share * at_once;
+  // piece 0 is slot 1 of its range, piece i slot 0 of range + i: rows (2 range + 1) ROWS, then 2 ROWS apart from + ROWS
+  const int row0 = (range * 2 + 1) * ROWS;
+  for (int row = row_in; row - row_in < rows; row += at_once) {
+    const bool live = share < shares && row < rows;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+      // pieces 1 + share, 1 + share + shares, .. and, of share 0, piece 0
+      if (share == 0) join_pieces<1>(p.part_o + c, p.part_ml, row0 + row, 0, 1, p.part_cols, m, l, acc);
+      join_pieces<8>(p.part_o + c, p.part_ml, row0 + row + ROWS + share * 2 * ROWS, shares * 2 * ROWS,
+                     (pieces - 1 - share + shares - 1) / shares, p.part_cols, m, l, acc);
+    }
+    if (shares > 1) {  // (then one round takes all rows)
+      __syncthreads();
+      s_acc[threadIdx.x] = acc;
+      s_ml[threadIdx.x] = make_float2(m, l);
+      __syncthreads();
+      if (share == 0)
+        for (int i = 1; i < shares; ++i) {
+          const int from = threadIdx.x + ((i * at_once) << shift);
+          join(m, l, acc, s_ml[from], s_acc[from]);
+        }
+    }
+    if (live && share == 0) {
+      const int r = it.y + row, tok = r / p.G;
+      store_row<T>(p, static_cast<int64_t>(it.x + tok) * p.H_q + head * p.G + r - tok * p.G, c, acc, m, l);
+    }
+  }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
-  constexpr int ROWS = kRows * MT, CH = DB / 4;
   __shared__ float4 s_acc[kMergeThreads];
   __shared__ float2 s_ml[kMergeThreads];
   pdl_launch_dependents();
   pdl_wait();
-  const int4 it = p.part_item[blockIdx.x];  // sequence, head, row tile, further pieces
-  if (it.w < 0) return;
-  const SeqLens sl = seq_lens(p.view, it.x);
-  const int rows = min(ROWS, sl.count * p.G - it.z * ROWS);
-  const int columns = rows * CH;
-  const int at_once = min(columns, kMergeThreads);
-  const int shares = columns < kMergeThreads ? kMergeThreads / columns : 1;
-  const int share = threadIdx.x / at_once, x = threadIdx.x - share * at_once;
-  // piece 0 is slot 1 of its range, the others are slot 0 of theirs
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 2 + 1) * ROWS;
-  for (int col0 = 0; col0 < columns; col0 += kMergeThreads) {
-    const int idx = col0 + x;
-    const int row = idx / CH, c = (idx - row * CH) * 4;
-    const bool live = share < shares && idx < columns;
-    float m = -INFINITY, l = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (live) {
-#pragma unroll 8
-      for (int i = share; i <= it.w; i += shares) {
-        const int64_t piece = first + row + (i ? ROWS + static_cast<int64_t>(i - 1) * 2 * ROWS : 0);
-        const float2 ml = p.part_ml[piece];
-        join(m, l, acc, ml, *reinterpret_cast<const float4*>(p.part_o + piece * DB + c));
-      }
-    }
-    if (shares > 1) {  // (then all columns fit one round)
-      s_acc[threadIdx.x] = acc;
-      s_ml[threadIdx.x] = make_float2(m, l);
-      __syncthreads();
-      if (share == 0) {
-        for (int i = 1; i < shares; ++i) join(m, l, acc, s_ml[i * at_once + x], s_acc[i * at_once + x]);
-      }
-    }
-    if (live && share == 0) {
-      const int r = it.z * ROWS + row;
-      store_row<T>(p, static_cast<int64_t>(sl.begin + r / p.G) * p.H_q + it.y * p.G + r % p.G, c, acc, m, l);
-    }
+  const int stride = gridDim.x;
+  constexpr int kAhead = 2;  // records a block reads at once
+  for (int i0 = blockIdx.x; i0 < p.part_ranges; i0 += kAhead * stride) {
+    int4 it[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) it[k] = i0 + k * stride < p.part_ranges ? p.part_item[i0 + k * stride] : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (it[k].z > 0) merge_range<T>(p, i0 + k * stride, it[k], s_acc, s_ml);
   }
 }
 

@@ -25,9 +25,8 @@
 // Work: an item is a pair of row tiles of one (sequence, KV head).  With at
 // least as many items as SMs they run whole, but for the last items % SMs,
 // which are cut into floor(SMs / rest) pieces each so that the last wave is
-// full too.  With fewer, each is cut in proportion to its sequence's length, to
-// about one piece an SM.  Pieces leave unnormalised sums that merge_kernel
-// joins.  Every CTA works the cut out itself from the lengths on the device.
+// full too.  With fewer, each is cut in proportion to its cost.  Pieces leave unnormalised sums that
+// merge_kernel joins.  Every CTA works the cut out itself from the lengths on the device.
 #pragma once
 #include "fwd_tc.cuh"
 #include "paged_mma.cuh"
@@ -84,7 +83,6 @@ __device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
       "r"(one)
       : "memory");
 }
-constexpr int kMergeThreads = 256;
 
 template <int DQK, int DV>
 struct Cfg {
@@ -167,74 +165,125 @@ struct Piece {
 __device__ __forceinline__ int pairs_of(const SeqLens& s, int tokens2) { return (s.count + tokens2 - 1) / tokens2; }
 __device__ __forceinline__ int tiles_of(const SeqLens& s) { return max(1, (s.held + kBN - 1) / kBN); }
 
-__device__ __forceinline__ int64_t warp_scan(int64_t x) {  // inclusive
+// Time of one of its items: a tile of 64 keys takes 1.15 us for a pair of row
+// tiles, 0.65 us where the tokens fill the first alone (D = 128).
+__device__ __forceinline__ float cost_of(const SeqLens& s, int tokens2) {
+  return static_cast<float>(tiles_of(s)) * (s.count > tokens2 / 2 ? 9.0f : 5.0f);
+}
+constexpr float kStart = 54.0f;  // what a piece costs beside its tiles
+// Pieces of an item: its cost in quanta, rounded (a piece costs from 2/3 to 3/2
+// of a quantum), and no more than its tiles.
+__device__ __forceinline__ int cuts_of(const SeqLens& s, int tokens2, float per_quantum) {
+  return max(1, min(tiles_of(s), static_cast<int>(cost_of(s, tokens2) * per_quantum + 0.5f)));
+}
+
+__device__ __forceinline__ int warp_scan(int x) {  // inclusive
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, x, d);
+    const int up = __shfl_up_sync(0xffffffffu, x, d);
     if ((threadIdx.x & 31) >= d) x += up;
   }
   return x;
 }
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
 
 // The piece that CTA `idx` computes; false if there is none.  Every warp works
-// it out for itself (no barrier): lane i takes the i-th share of the sequences.
-// slots: workspace slots of the call.
-__device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, Piece& out, int& slots) {
+// it out for itself (no barrier, and the same everywhere): lane i takes the
+// i-th share of the sequences.  slots: workspace slots of the call.  (Items and
+// pieces are counted in 32 bits; the host refuses more.)
+__device__ __forceinline__ bool find_piece(const Params& p, int idx, Piece& out, int& slots) {
   const int lane = threadIdx.x & 31;
   const int tokens2 = 2 * (kBM / p.G);
   const int per = (p.view.seqs + 31) / 32, n0 = lane * per, n1 = min(p.view.seqs, n0 + per);
-  int64_t items = 0, work = 0;
-  for (int n = n0; n < n1; ++n) {
-    const SeqLens s = seq_lens(p.view, n);
-    const int64_t pr = pairs_of(s, tokens2);
-    items += pr;
-    work += pr * tiles_of(s);
-  }
-  const int64_t items_to = warp_scan(items);
-  const int64_t all_items = __shfl_sync(0xffffffffu, items_to, 31) * p.H_kv;
-  const int64_t sms = p.sms;
-  const bool whole = all_items >= sms;  // the first `full` items run whole
-  int64_t target = idx, at = (items_to - items) * p.H_kv;  // first item (piece) of this lane's sequences
-  int64_t full = 0, quantum = 1;
-  int cut = 1, piece = 0;
+  const SeqLens none = {0, 0, 0};
+  const SeqLens s0 = n0 < n1 ? seq_lens(p.view, n0) : none;  // (the only one, up to 32 sequences)
+  auto lens = [&](int n) { return n == n0 ? s0 : seq_lens(p.view, n); };
+  int items = 0;
+  for (int n = n0; n < n1; ++n) items += pairs_of(lens(n), tokens2);
+  const int items_to = warp_scan(items);
+  const int all_items = __shfl_sync(0xffffffffu, items_to, 31) * p.H_kv;
+  const bool whole = all_items >= p.sms;  // the first `full` items run whole
+  int target = idx, at = (items_to - items) * p.H_kv;  // first item (piece) of this lane's sequences
+  int full = 0, cut = 1, piece = 0;
+  float per_quantum = 0.0f;
   if (whole) {
-    const int rest = static_cast<int>(all_items % sms);
+    const int rest = all_items % p.sms;
     full = all_items - rest;
     const int cuts = rest ? p.sms / rest : 1;
     slots = cuts > 1 ? rest * cuts : 0;
     if (idx >= full) {
       cut = cuts;
       target = full + (idx - full) / cut;
-      piece = static_cast<int>((idx - full) % cut);
+      piece = (idx - full) % cut;
     }
   } else {
-    const int64_t all_work = __shfl_sync(0xffffffffu, warp_scan(work), 31) * p.H_kv;
-    quantum = max(static_cast<int64_t>(1), (all_work + sms - 1) / sms);
-    int64_t mine = 0;
-    for (int n = n0; n < n1; ++n) {
-      const SeqLens s = seq_lens(p.view, n);
-      mine += static_cast<int64_t>(pairs_of(s, tokens2)) * max(static_cast<int64_t>(1), tiles_of(s) / quantum);
+    float work = 0.0f;
+    for (int n = n0; n < n1; ++n) work += static_cast<float>(pairs_of(lens(n), tokens2)) * cost_of(lens(n), tokens2);
+    const float heads = static_cast<float>(p.H_kv), sms = static_cast<float>(p.sms);
+    const float all = warp_sum(work) * heads;
+    // The quantum, from 4/5 to 2 even shares of the SMs, whose pieces are
+    // expected to end first: in one wave, the longest piece; in more, an even
+    // share and half a piece.
+    float best = INFINITY;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const float pq = sms / (all * (k == 0 ? 0.8f : k == 1 ? 1.0f : k == 2 ? 1.3f : 2.0f));
+      float pieces = 0.0f, longest = 0.0f;
+      for (int n = n0; n < n1; ++n) {
+        const SeqLens s = lens(n);
+        const float cuts = static_cast<float>(cuts_of(s, tokens2, pq));
+        pieces += static_cast<float>(pairs_of(s, tokens2)) * cuts;
+        if (s.count > 0) longest = fmaxf(longest, __fdividef(cost_of(s, tokens2), cuts));
+      }
+      pieces = warp_sum(pieces) * heads;
+      float time = warp_max(longest) + kStart;
+      if (pieces > sms) time = fmaxf(time, __fdividef(all + pieces * kStart, sms) + 0.5f * (__fdividef(all, pieces) + kStart));
+      if (time < best) best = time, per_quantum = pq;
     }
-    const int64_t to = warp_scan(mine);
-    at = (to - mine) * p.H_kv;
-    slots = static_cast<int>(__shfl_sync(0xffffffffu, to, 31) * p.H_kv);
+    int mine = 0;
+    float cost = 0.0f;
+    for (int n = n0; n < n1; ++n) {
+      const int cuts = cuts_of(lens(n), tokens2, per_quantum);
+      mine += pairs_of(lens(n), tokens2) * cuts;
+      cost = __fdividef(cost_of(lens(n), tokens2), static_cast<float>(cuts));
+    }
+    const int to = warp_scan(mine);
+    slots = __shfl_sync(0xffffffffu, to, 31) * p.H_kv;
+    at = to - mine;
+    if (per == 1 && p.view.seqs > 1) {  // a sequence a lane: the longest pieces first, so that short ones fill the last gaps
+      at = 0;
+      for (int k = 0; k < p.view.seqs; ++k) {
+        const float c = __shfl_sync(0xffffffffu, cost, k);
+        const int m = __shfl_sync(0xffffffffu, mine, k);
+        if (c > cost || (c == cost && k < lane)) at += m;
+      }
+    }
+    at *= p.H_kv;
   }
   bool found = false;
   Piece f = {0, 0, 0, 0, 1, 0};
   for (int n = n0; n < n1; ++n) {
-    const SeqLens s = seq_lens(p.view, n);
-    const int64_t pr = pairs_of(s, tokens2);
-    if (!whole) cut = static_cast<int>(max(static_cast<int64_t>(1), tiles_of(s) / quantum));
-    const int64_t count = pr * p.H_kv * (whole ? 1 : cut);
+    const int pr = pairs_of(lens(n), tokens2);
+    if (!whole) cut = cuts_of(lens(n), tokens2, per_quantum);
+    const int count = pr * p.H_kv * (whole ? 1 : cut);
     if (target >= at && target < at + count) {
-      int64_t local = target - at;
+      int local = target - at;
       if (!whole) {
-        piece = static_cast<int>(local % cut);
+        piece = local % cut;
         local /= cut;
       }
       f.seq = n;
-      f.head = static_cast<int>(local / pr);
-      f.pair = static_cast<int>(pr - 1 - local % pr);  // longest causal rows first
+      f.head = local / pr;
+      f.pair = pr - 1 - (local - f.head * pr);  // longest causal rows first
       f.piece = piece;
       f.pieces = cut;
       found = true;
@@ -249,7 +298,7 @@ __device__ __forceinline__ bool find_piece(const Params& p, int64_t idx, Piece& 
   out.pair = __shfl_sync(0xffffffffu, f.pair, src);
   out.piece = __shfl_sync(0xffffffffu, f.piece, src);
   out.pieces = __shfl_sync(0xffffffffu, f.pieces, src);
-  out.slot = static_cast<int>(idx - full);
+  out.slot = idx - full;
   return true;
 }
 
@@ -307,33 +356,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     bars->abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(&bars->tmem_base, C::kTmemCols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  __syncthreads();  // (the barriers are set up)
   pdl_launch_dependents();
   pdl_wait();  // before any global access and before the wait deadline starts
-  const uint32_t tmem = bars->tmem_base;
+  Piece w;
+  int slots;
+  const bool live = find_piece(p, static_cast<int>(blockIdx.x), w, slots);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.tc_slots = slots;
+  if (!live) return;
   WaitCtl ctl;
   ctl.deadline_ns = globaltimer_ns() + p.timeout_ns;
   ctl.abort_flag = &bars->abort_flag;
-  Piece w;
-  int slots;
-  const bool live = find_piece(p, blockIdx.x, w, slots);
-  // what merge_kernel goes by: the slots, and of each slot its item (pieces in .w where it is the first of several)
-  if (threadIdx.x == 0) {
-    if (blockIdx.x == 0) *p.part_slots = slots;
-    if (live && w.slot >= 0 && w.slot < slots)
-      p.part_item[w.slot] = make_int4(w.seq, w.head, w.pair, w.piece == 0 && w.pieces > 1 ? w.pieces : 0);
+  uint32_t tmem = 0;
+  if (warp == 9) tmem_alloc(&bars->tmem_base, C::kTmemCols);
+  if (warp != 8 && warp != 11) {  // (the TMA warps go ahead)
+    tc_fence_before();
+    asm volatile("bar.sync 1, 320;" ::: "memory");
+    tc_fence_after();
+    tmem = bars->tmem_base;
   }
-  if (!live) {
-    if (warp == 9) tmem_dealloc(tmem, C::kTmemCols);
-    return;
-  }
-
   const SeqLens sl = seq_lens(p.view, w.seq);
   const Range rg = range_of(p, sl, w);
   const int tpt = kBM / p.G;  // tokens of a row tile
+  // what merge_kernel goes by, of each slot
+  if (threadIdx.x == 0 && w.slot >= 0 && w.slot < slots)
+    p.tc_item[w.slot] = make_int4(sl.begin + rg.tok0, min(2 * tpt, sl.count - rg.tok0), w.head,
+                                  w.pieces << 16 | w.piece);
   const int n_kv = rg.j1 - rg.j0;
   // key tiles per row tile within the piece; the second tile may have no tokens
   int n_t[2];
@@ -594,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float mul = part ? f : (l_true > kEps ? f / l_true : 0.0f);
       if (active) {
         if (part)
-          p.part_ml[prow] = make_float2(m_run, l_true);
+          p.tc_ml[prow] = make_float2(m_run, l_true);
         else
           p.stats[row] = (m_run == -INFINITY ? kNegInit : m_run * kLn2) + logf(l_true + kEps);
       }
@@ -614,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; ++e) x[e] = mul == 0.0f ? 0.0f : __uint_as_float(o[e]) * mul;
         if (active) {
           if (part) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * DV + c * 32);
+            float4* dst = reinterpret_cast<float4*>(p.tc_o + prow * DV + c * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
           } else {
@@ -639,41 +687,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the cut items.  Units of kMergeRows rows of one slot's
-// item go round the CTAs; a thread adds one float4 column of one row over the
-// pieces.
-constexpr int kMergeRows = 32;
-constexpr int kUnits = 2 * kBM / kMergeRows;  // of a slot
-
+// Joins the pieces of cut items: every slot's share of its item's rows, in
+// quarters, go round the blocks in turn.
 template <int DV>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
-  constexpr int CH = DV / 4;
+__global__ void __launch_bounds__(paged::kMergeThreads) merge_kernel(const Params p) {
+  constexpr int kRowsOfItem = 2 * kBM, CH = DV / 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int units = *p.part_slots * kUnits, tpt = kBM / p.G;
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int slot = unit / kUnits;
-    const int4 it = p.part_item[slot];
-    if (it.w == 0) continue;
-    const SeqLens sl = seq_lens(p.view, it.x);
-    const int tok0 = it.z * 2 * tpt;
-    for (int i = threadIdx.x; i < kMergeRows * CH; i += kMergeThreads) {
-      const int row = (unit % kUnits) * kMergeRows + i / CH, c = (i % CH) * 4;
-      const int r_in = row % kBM, tok = tok0 + row / kBM * tpt + r_in / p.G;
-      if (r_in >= tpt * p.G || tok >= sl.count) continue;
-      const int64_t first = static_cast<int64_t>(slot) * (2 * kBM) + row;
+  const int c = (threadIdx.x % CH) * 4;
+  const int units = *p.tc_slots * 4, tpt = kBM / p.G;
+  const float inv = 1.0f / static_cast<float>(p.G);
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int slot = u / 4;
+    const int4 it = p.tc_item[slot];
+    const int pieces = it.w >> 16, mine = it.w & 0xffff;
+    if (pieces < 2) continue;
+    const int parts = 4 * pieces, part = 4 * mine + u % 4;
+    const int begin = kRowsOfItem * part / parts, end = kRowsOfItem * (part + 1) / parts;
+    for (int row = begin + threadIdx.x / CH; row < end; row += paged::kMergeThreads / CH) {
+      const int r_in = row & 127;
+      const int in_tile = static_cast<int>((static_cast<float>(r_in) + 0.5f) * inv);  // r_in / G, exact below 128
+      const int tok = (row >> 7) * tpt + in_tile;                                      // of the pair's tokens
+      if (r_in >= tpt * p.G || tok >= it.y) continue;
       float m = -INFINITY, l = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-      for (int k = 0; k < it.w; ++k) {
-        const float2 a = p.part_ml[first + k * 2 * kBM];
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (first + k * 2 * kBM) * DV + c);
-        paged::join(m, l, acc, a, x);
-      }
-      paged::store_row<__half>(p, static_cast<int64_t>(sl.begin + tok) * p.H_q + it.y * p.G + r_in % p.G, c, acc, m, l);
+      paged::join_pieces<4>(p.tc_o + c, p.tc_ml, (slot - mine) * kRowsOfItem + row, kRowsOfItem, pieces, DV, m, l, acc);
+      paged::store_row<__half>(p, static_cast<int64_t>(it.x + tok) * p.H_q + it.z * p.G + r_in - in_tile * p.G, c, acc, m, l);
     }
   }
 }
+
 
 }  // namespace paged_tc
 }  // namespace sdpa_b200
