@@ -6,12 +6,16 @@
 // Backward: g = R(pos)^T dy,  dw = sum g * n,  dx = rsqrt(..) * (g w - n * mean(g w n)).
 //
 // Bound: HBM bytes (forward: x in, y out; backward: x, dy in, dx out); per
-// element ~10 fp32 operations.  One group of LANES lanes owns one head row,
-// eight features a lane, so the row's sum is three or four shuffles and both
-// members of every rotated pair sit in one lane: for pairs (i, i + rot/2) a lane
-// holds features 4j.. and rot/2 + 4j.., for neighbouring pairs 8j..8j+7.  A
-// group walks several heads of one token with the token's cosines and sines in
-// registers, four heads at a time (eight loads in flight a lane).
+// element about ten fp32 operations, so the work beside the loads is kept short:
+// a group of LANES lanes owns one head row, eight features a lane, so the row's
+// sum is three or four shuffles; both members of every rotated pair sit in one
+// lane (for pairs (i, i + rot/2) features 4j.. and rot/2 + 4j.., for neighbouring
+// pairs 8j..), weights, cosines and sines are multiplied once a token, and the
+// products go in packed pairs (f32x2).  A group walks the heads of one token,
+// four at a time with all their loads ahead of the arithmetic.  32768 tokens x
+// 32 heads x 128 in fp16: forward 108 us (537 MB, 5.0 TB/s), backward 200 us (805 MB,
+// 4.0 TB/s); with the weights and the turn apart 120 and 215 us; sixteen features a
+// lane (16-byte loads, fewer instructions, but over 110 registers) 118 and 205 us.
 // All arithmetic is fp32, rounded to T once, at the store.
 #pragma once
 #include "common.cuh"
@@ -22,8 +26,8 @@ namespace sdpa_b200 {
 namespace rotary {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;        // heads a group has in flight
-constexpr int kGradBlocks = 592; // most token blocks of the backward (rows of its workspace)
+constexpr int E = 4;              // features of one of a lane's two runs
+constexpr int kGradBlocks = 592;  // most blocks of the backward (rows of its workspace)
 
 // One of q, k (or v, copied as it is).
 struct Stream {
@@ -40,7 +44,7 @@ struct Params {
   Stream q, k, v;
   int D, D_v;
   int weight_f32;      // weights are float32 (else T)
-  float eps;
+  float eps, inv_D;    // inv_D = 1 / D
   const float* table;  // [max_positions, rot]: cos | sin; null: no rotation
   int max_positions, rot, interleaved;
   // cache write
@@ -54,97 +58,122 @@ struct Params {
   int blocks;
 };
 
+// E consecutive features as loaded, and as floats.
 template <typename T>
-struct Vec4;
-template <>
-struct Vec4<float> {
-  using type = float4;
-  static __device__ __forceinline__ void unpack(const float4& r, float* x) { x[0] = r.x, x[1] = r.y, x[2] = r.z, x[3] = r.w; }
-  static __device__ __forceinline__ float4 pack(const float* x) { return make_float4(x[0], x[1], x[2], x[3]); }
-};
-template <>
-struct Vec4<__half> {
-  using type = uint2;
-  static __device__ __forceinline__ void unpack(const uint2& r, float* x) {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+struct Raw {
+  uint32_t w[E * sizeof(T) / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if (sizeof(w) == 8) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = x.x, w[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+      }
+    }
   }
-  static __device__ __forceinline__ uint2 pack(const float* x) {
-    return make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+  __device__ __forceinline__ void store(T* p) const {
+    if (sizeof(w) == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(w) / 4); ++i) {
+      if (sizeof(T) == 2) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = x.x, f[2 * i + 1] = x.y;
+      } else {
+        f[i] = __uint_as_float(w[i]);
+      }
+    }
+  }
+  __device__ __forceinline__ void pack(const float* f) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(w) / 4); ++i)
+      w[i] = sizeof(T) == 2 ? pack_half2(f[2 * i], f[2 * i + 1]) : __float_as_uint(f[i]);
   }
 };
 
-// Where a lane's eight features lie and how they turn.
+// Where a lane's features lie, two runs of E, and whether they turn.
+template <bool INTER>
 struct Place {
-  int a, b;           // first feature of its two groups of four
+  int a, b;           // first feature of each run
+  int angle;          // of its E pairs: index of the first
   bool live, turned;  // inside the row; inside the rotated part
+  __device__ __forceinline__ Place(int lane, const Params& p) {
+    live = lane * 2 * E < p.D;
+    turned = p.table && lane * 2 * E < p.rot;
+    const bool halves = turned && !INTER;
+    a = halves ? lane * E : lane * 2 * E;
+    b = halves ? p.rot / 2 + lane * E : lane * 2 * E + E;
+    angle = lane * E;
+  }
+  // registers of pair e's members
+  static __device__ __forceinline__ constexpr int first(int e) { return INTER ? 2 * e : e; }
+  static __device__ __forceinline__ constexpr int second(int e) { return INTER ? 2 * e + 1 : E + e; }
 };
-__device__ __forceinline__ Place place_of(int lane, const Params& p) {
-  Place c;
-  c.live = lane * 8 < p.D;
-  c.turned = p.table && lane * 8 < p.rot;
-  const bool halves = c.turned && !p.interleaved;
-  c.a = halves ? lane * 4 : lane * 8;
-  c.b = halves ? p.rot / 2 + lane * 4 : lane * 8 + 4;
-  return c;
-}
 
-template <typename T>
-__device__ __forceinline__ void load_weight(const void* w, int f32, const Place& c, float* out) {
-  if (!w || !c.live) {
+template <typename T, bool INTER>
+__device__ __forceinline__ void load_weight(const void* w, int f32, const Place<INTER>& c, float* out) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = 1.0f;
-    return;
-  }
-  if (f32) {
-    const float* f = static_cast<const float*>(w);
+  for (int e = 0; e < 2 * E; ++e) out[e] = 1.0f;
+  if (!w || !c.live) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = f[c.a + e], out[4 + e] = f[c.b + e];
-  } else {
-    const T* f = static_cast<const T*>(w);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = to_f<T>(f[c.a + e]), out[4 + e] = to_f<T>(f[c.b + e]);
+  for (int e = 0; e < E; ++e) {
+    out[e] = f32 ? static_cast<const float*>(w)[c.a + e] : to_f<T>(static_cast<const T*>(w)[c.a + e]);
+    out[E + e] = f32 ? static_cast<const float*>(w)[c.b + e] : to_f<T>(static_cast<const T*>(w)[c.b + e]);
   }
 }
 
-// Cosines and sines of a lane's four pairs at `pos` (1 and 0 where nothing turns).
-__device__ __forceinline__ void load_turn(const Params& p, const Place& c, int lane, int64_t pos, float* cs, float* sn) {
+// Cosines and sines of a lane's E pairs at `pos` (1 and 0 where nothing turns).
+template <bool INTER>
+__device__ __forceinline__ void load_turn(const Params& p, const Place<INTER>& c, int lane, int64_t pos, float* cs,
+                                          float* sn) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+  for (int e = 0; e < E; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
   if (!p.table) return;
   if (pos < 0 || pos >= p.max_positions) {
     if (lane == 0) atomicOr(&g_status_word, kStatusBadIndex);
     pos = pos < 0 ? 0 : p.max_positions - 1;
   }
   if (c.turned) {
-    const float* row = p.table + pos * p.rot + lane * 4;
-    const float4 a = __ldg(reinterpret_cast<const float4*>(row));
-    const float* srow = row + p.rot / 2;
-    const float4 b = __ldg(reinterpret_cast<const float4*>(srow));
-    cs[0] = a.x, cs[1] = a.y, cs[2] = a.z, cs[3] = a.w;
-    sn[0] = b.x, sn[1] = b.y, sn[2] = b.z, sn[3] = b.w;
+    const float* row = p.table + pos * p.rot + c.angle;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(row + e));
+      cs[e] = a.x, cs[e + 1] = a.y, cs[e + 2] = a.z, cs[e + 3] = a.w;
+    }
+    const float* srow = row + p.rot / 2;  // (a multiple of four floats)
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(srow + e));
+      sn[e] = b.x, sn[e + 1] = b.y, sn[e + 2] = b.z, sn[e + 3] = b.w;
+    }
   }
 }
 
-// x <- R x (sign = 1) or R^T x (sign = -1) on a lane's eight features.
-__device__ __forceinline__ void turn(float* x, const float* cs, const float* sn, bool interleaved, float sign) {
-  if (interleaved) {
+// The turn of weighted features, y = R (x w): first = x1 ca - x2 sb, second = x2 cb + x1 sa.
+struct Turn {
+  float ca[E], sb[E], cb[E], sa[E];
+  template <bool INTER>
+  __device__ __forceinline__ void set(const float* w, const float* cs, const float* sn) {
+    using P = Place<INTER>;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = x[2 * e], b = x[2 * e + 1], s = sign * sn[e];
-      x[2 * e] = a * cs[e] - b * s;
-      x[2 * e + 1] = b * cs[e] + a * s;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = x[e], b = x[4 + e], s = sign * sn[e];
-      x[e] = a * cs[e] - b * s;
-      x[4 + e] = b * cs[e] + a * s;
+    for (int e = 0; e < E; ++e) {
+      ca[e] = w[P::first(e)] * cs[e];
+      sa[e] = w[P::first(e)] * sn[e];
+      cb[e] = w[P::second(e)] * cs[e];
+      sb[e] = -w[P::second(e)] * sn[e];
     }
   }
-}
+};
 
 template <int LANES>
 __device__ __forceinline__ float group_sum(float x, unsigned mask) {
@@ -153,39 +182,61 @@ __device__ __forceinline__ float group_sum(float x, unsigned mask) {
   return x;
 }
 
-// Heads [h0, h0 + kHeads) of one token's row: norm, rotation, store.
-template <typename T, int LANES>
-__device__ __forceinline__ void forward_heads(const T* x, T* y, int heads, int h0, const Params& p, const Place& c,
-                                              const float* w, bool norm, const float* cs, const float* sn,
-                                              unsigned mask) {
-  using V = Vec4<T>;
-  typename V::type ra[kHeads], rb[kHeads];
+// Heads [h0, h0 + N) of one token's row: norm, rotation, store.
+template <typename T, int LANES, bool INTER, int N>
+__device__ __forceinline__ void forward_heads(const T* x, T* y, int heads, int h0, const Params& p,
+                                              const Place<INTER>& c, const Turn& w, bool norm, unsigned mask) {
+  using P = Place<INTER>;
+  Raw<T> ra[N], rb[N];
+  const T *xa = x + h0 * p.D + c.a, *xb = x + h0 * p.D + c.b;
+  T *ya = y + h0 * p.D + c.a, *yb = y + h0 * p.D + c.b;
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i)
-    if (c.live && h0 + i < heads) {
-      ra[i] = __ldg(reinterpret_cast<const typename V::type*>(x + (h0 + i) * p.D + c.a));
-      rb[i] = __ldg(reinterpret_cast<const typename V::type*>(x + (h0 + i) * p.D + c.b));
-    }
+  for (int i = 0; i < N; ++i)
+    if (c.live && h0 + i < heads) ra[i].load(xa + i * p.D), rb[i].load(xb + i * p.D);
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
+  for (int i = 0; i < N; ++i) {
     if (h0 + i >= heads) break;  // the same for every lane of the group
-    float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (c.live) V::unpack(ra[i], f), V::unpack(rb[i], f + 4);
+    float f[2 * E];
+#pragma unroll
+    for (int e = 0; e < 2 * E; ++e) f[e] = 0.0f;
+    if (c.live) ra[i].unpack(f), rb[i].unpack(f + E);
+    float r = 1.0f;
     if (norm) {
-      float ss = 0.0f;
+      float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-      const float r = rsqrtf(group_sum<LANES>(ss, mask) / static_cast<float>(p.D) + p.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= r * w[e];
+      for (int e = 0; e < 2 * E; e += 2) ffma2(s0, s1, f[e], f[e + 1], f[e], f[e + 1], s0, s1);
+      r = rsqrtf(group_sum<LANES>(s0 + s1, mask) * p.inv_D + p.eps);
     }
-    turn(f, cs, sn, p.interleaved, 1.0f);
+    float z[2 * E];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      float u0, u1, v0, v1;
+      const float a0 = f[P::first(e)], a1 = f[P::first(e + 1)], b0 = f[P::second(e)], b1 = f[P::second(e + 1)];
+      fmul2(u0, u1, a0, a1, w.ca[e], w.ca[e + 1]);
+      ffma2(u0, u1, b0, b1, w.sb[e], w.sb[e + 1], u0, u1);
+      fmul2(v0, v1, b0, b1, w.cb[e], w.cb[e + 1]);
+      ffma2(v0, v1, a0, a1, w.sa[e], w.sa[e + 1], v0, v1);
+      fmul2(z[P::first(e)], z[P::first(e + 1)], u0, u1, r, r);
+      fmul2(z[P::second(e)], z[P::second(e + 1)], v0, v1, r, r);
+    }
     if (c.live) {
-      *reinterpret_cast<typename V::type*>(y + (h0 + i) * p.D + c.a) = V::pack(f);
-      *reinterpret_cast<typename V::type*>(y + (h0 + i) * p.D + c.b) = V::pack(f + 4);
+      Raw<T> o;
+      o.pack(z);
+      o.store(ya + i * p.D);
+      o.pack(z + E);
+      o.store(yb + i * p.D);
     }
   }
 }
+
+constexpr int kHeadsAhead = 4;  // heads a group has in flight
+// Blocks an SM (fp16: 64 registers a thread; fp32 holds twice the loads).  At
+// 64 the append kernel spills some addresses and gains all the same: 38 us
+// against 46 for 5251 tokens x 48 heads x 128.
+template <typename T>
+constexpr int kBlocks = sizeof(T) == 2 ? 4 : 3;
+// Head groups of a stream.
+__host__ __device__ __forceinline__ int units_of(int heads, int ahead) { return (heads + ahead - 1) / ahead; }
 
 // Token t of one stream: the head groups u of [u0, units) this block row takes.
 template <int LANES>
@@ -202,44 +253,53 @@ struct Group {
 
 // grid.x: blocks of kThreads / LANES tokens; grid.y: shares of a token's head
 // groups (more of them when there are few tokens).
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
+template <typename T, int LANES, bool INTER>
+__global__ void __launch_bounds__(kThreads, kBlocks<T>) forward_kernel(const Params p) {
+  constexpr int N = kHeadsAhead;
   pdl_launch_dependents();
   const Group<LANES> g;
-  const Place c = place_of(g.lane, p);
+  const Place<INTER> c(g.lane, p);
   pdl_wait();
-  const int uq = (p.q.heads + kHeads - 1) / kHeads, uk = (p.k.heads + kHeads - 1) / kHeads;
+  const int uq = units_of(p.q.heads, N), uk = units_of(p.k.heads, N);
   const int64_t tokens = max(p.q.tokens, p.k.tokens);
   if (g.token >= tokens) return;
-  float cs[4], sn[4], w[8];
-  int64_t at = -1;  // the position cs, sn were read for
-  int kind = -1;    // the stream w was read for
+  Turn turn;
+  int64_t at = -1;  // the position and stream that `turn` is of
+  int kind = -1;
   for (int u = blockIdx.y; u < uq + uk; u += gridDim.y) {
     const bool is_k = u >= uq;
     const Stream& s = is_k ? p.k : p.q;
     if (g.token >= s.tokens) continue;
-    const int64_t pos = s.positions ? s.positions[g.token] : g.token % s.period;
-    if (kind < 0 || pos != at) load_turn(p, c, g.lane, pos, cs, sn), at = pos;
-    if (kind != (is_k ? 1 : 0)) load_weight<T>(s.weight, p.weight_f32, c, w), kind = is_k ? 1 : 0;
-    forward_heads<T, LANES>(static_cast<const T*>(s.x) + g.token * s.stride,
-                            static_cast<T*>(s.y) + g.token * s.heads * p.D, s.heads, (is_k ? u - uq : u) * kHeads, p, c,
-                            w, s.weight != nullptr, cs, sn, g.mask);
+    const int64_t pos = s.positions ? s.positions[g.token] : static_cast<int>(g.token) % s.period;
+    if (kind != (is_k ? 1 : 0) || pos != at) {
+      float cs[E], sn[E], w[2 * E];
+      load_turn(p, c, g.lane, pos, cs, sn);
+      load_weight<T>(s.weight, p.weight_f32, c, w);
+      turn.set<INTER>(w, cs, sn);
+      kind = is_k ? 1 : 0;
+      at = pos;
+    }
+    forward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + g.token * s.stride,
+                                         static_cast<T*>(s.y) + g.token * s.heads * p.D, s.heads, (is_k ? u - uq : u) * N,
+                                         p, c, turn, s.weight != nullptr, g.mask);
   }
 }
 
 // The cache write: keys to their page row, queries (if any) to q.y, values
 // copied.  Tokens behind the last sequence, at positions below zero or past
 // the table, and on pages outside the pool are not written.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
+constexpr int kCopyWords = 4;  // 16-byte words of the values a lane has in flight
+template <typename T, int LANES, bool INTER>
+__global__ void __launch_bounds__(kThreads, kBlocks<T>) append_kernel(const Params p) {
+  constexpr int N = kHeadsAhead;
   pdl_launch_dependents();
   const Group<LANES> g;
-  const Place c = place_of(g.lane, p);
+  const Place<INTER> c(g.lane, p);
   constexpr int kVec = 16 / sizeof(T);
   pdl_wait();
-  const int uq = (p.q.heads + kHeads - 1) / kHeads, uk = (p.k.heads + kHeads - 1) / kHeads;
+  const int uq = units_of(p.q.heads, N), uk = units_of(p.k.heads, N);
   const int nv = p.k.heads * p.D_v / kVec;  // a token's values in 16-byte words, contiguous on both sides
-  const int uv = (nv + LANES * kHeads - 1) / (LANES * kHeads);
+  const int uv = units_of(nv, LANES * kCopyWords);
   if (g.token >= p.view.tokens) return;
   const int n = seq_of_token<LANES>(p.view, static_cast<int>(g.token), g.mask, g.lane);
   if (n < 0) return;
@@ -249,120 +309,144 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
   const int page = in_table ? page_of(p.view, n, static_cast<int>(pos >> p.view.page_shift)) : -1;
   if (!in_table && g.lane == 0) atomicOr(&g_status_word, kStatusBadIndex);
   const int64_t slot = (static_cast<int64_t>(page) << p.view.page_shift) + (pos & ((1 << p.view.page_shift) - 1));
-  float cs[4], sn[4], w[8];
+  float cs[E], sn[E];
   load_turn(p, c, g.lane, pos, cs, sn);
-  int kind = -1;
+  Turn turn;
+  int kind = -1;  // the stream that `turn` is of
   for (int u = blockIdx.y; u < uq + uk + uv; u += gridDim.y) {
     if (u >= uq + uk) {
       if (page < 0) continue;
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.x) + g.token * p.v.stride);
       uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.v_pages) + slot * p.k.heads * p.D_v);
-      const int i0 = (u - uq - uk) * LANES * kHeads + g.lane;
-      uint4 r[kHeads];
+      const int i0 = (u - uq - uk) * LANES * kCopyWords + g.lane;
+      uint4 r[kCopyWords];
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i)
+      for (int i = 0; i < kCopyWords; ++i)
         if (i0 + i * LANES < nv) r[i] = __ldg(src + i0 + i * LANES);
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i)
+      for (int i = 0; i < kCopyWords; ++i)
         if (i0 + i * LANES < nv) dst[i0 + i * LANES] = r[i];
       continue;
     }
     const bool is_k = u >= uq;
     if (is_k && page < 0) continue;
     const Stream& s = is_k ? p.k : p.q;
-    if (kind != (is_k ? 1 : 0)) load_weight<T>(s.weight, p.weight_f32, c, w), kind = is_k ? 1 : 0;
+    if (kind != (is_k ? 1 : 0)) {
+      float w[2 * E];
+      load_weight<T>(s.weight, p.weight_f32, c, w);
+      turn.set<INTER>(w, cs, sn);
+      kind = is_k ? 1 : 0;
+    }
     T* y = is_k ? static_cast<T*>(p.k_pages) + slot * s.heads * p.D : static_cast<T*>(s.y) + g.token * s.heads * p.D;
-    forward_heads<T, LANES>(static_cast<const T*>(s.x) + g.token * s.stride, y, s.heads, (is_k ? u - uq : u) * kHeads, p,
-                            c, w, s.weight != nullptr, cs, sn, g.mask);
+    forward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + g.token * s.stride, y, s.heads,
+                                         (is_k ? u - uq : u) * N, p, c, turn, s.weight != nullptr, g.mask);
   }
 }
 
-// Backward.  A block walks tokens blockIdx.x, + gridDim.x, ... of its group
-// index and all heads, summing dw in registers; the block's sums go to
-// partial[block][q, k][D], added by weight_kernel in block order (no atomics:
-// the same bits every run).
-constexpr int kGradHeads = 2;  // x and dy of two heads in flight
-
-template <typename T, int LANES>
+// Backward, heads [h0, h0 + N) of one token's row: dx, and dw summed.
+template <typename T, int LANES, bool INTER, int N>
 __device__ __forceinline__ void backward_heads(const T* x, const T* dy, T* dx, int heads, int h0, const Params& p,
-                                               const Place& c, const float* w, bool norm, const float* cs,
+                                               const Place<INTER>& c, const float* w, bool norm, const float* cs,
                                                const float* sn, unsigned mask, float* dw) {
-  using V = Vec4<T>;
-  typename V::type xa[kGradHeads], xb[kGradHeads], ga[kGradHeads], gb[kGradHeads];
+  using P = Place<INTER>;
+  Raw<T> xa[N], xb[N], ga[N], gb[N];
 #pragma unroll
-  for (int i = 0; i < kGradHeads; ++i)
+  for (int i = 0; i < N; ++i)
     if (c.live && h0 + i < heads) {
-      if (norm) {
-        xa[i] = __ldg(reinterpret_cast<const typename V::type*>(x + (h0 + i) * p.D + c.a));
-        xb[i] = __ldg(reinterpret_cast<const typename V::type*>(x + (h0 + i) * p.D + c.b));
-      }
-      ga[i] = __ldg(reinterpret_cast<const typename V::type*>(dy + (h0 + i) * p.D + c.a));
-      gb[i] = __ldg(reinterpret_cast<const typename V::type*>(dy + (h0 + i) * p.D + c.b));
+      if (norm) xa[i].load(x + (h0 + i) * p.D + c.a), xb[i].load(x + (h0 + i) * p.D + c.b);
+      ga[i].load(dy + (h0 + i) * p.D + c.a), gb[i].load(dy + (h0 + i) * p.D + c.b);
     }
 #pragma unroll
-  for (int i = 0; i < kGradHeads; ++i) {
+  for (int i = 0; i < N; ++i) {
     if (h0 + i >= heads) break;
-    float g[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (c.live) V::unpack(ga[i], g), V::unpack(gb[i], g + 4);
-    turn(g, cs, sn, p.interleaved, -1.0f);
+    float d[2 * E], g[2 * E];
+#pragma unroll
+    for (int e = 0; e < 2 * E; ++e) d[e] = 0.0f;
+    if (c.live) ga[i].unpack(d), gb[i].unpack(d + E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {  // g = R^T dy
+      const float a0 = d[P::first(e)], a1 = d[P::first(e + 1)], b0 = d[P::second(e)], b1 = d[P::second(e + 1)];
+      float u0, u1, v0, v1;
+      fmul2(u0, u1, a0, a1, cs[e], cs[e + 1]);
+      ffma2(g[P::first(e)], g[P::first(e + 1)], b0, b1, sn[e], sn[e + 1], u0, u1);
+      fmul2(v0, v1, b0, b1, cs[e], cs[e + 1]);
+      ffma2(g[P::second(e)], g[P::second(e + 1)], a0, a1, -sn[e], -sn[e + 1], v0, v1);
+    }
     if (norm) {
-      float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      if (c.live) V::unpack(xa[i], f), V::unpack(xb[i], f + 4);
+      float f[2 * E], gw[2 * E];
+#pragma unroll
+      for (int e = 0; e < 2 * E; ++e) f[e] = 0.0f;
+      if (c.live) xa[i].unpack(f), xb[i].unpack(f + E);
       // both sums at once: mean(g w n) = r * mean(g w x)
-      float ss = 0.0f, gx = 0.0f;
+      float s0 = 0.0f, s1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss), gx = fmaf(g[e] * w[e], f[e], gx);
-      ss = group_sum<LANES>(ss, mask);
-      gx = group_sum<LANES>(gx, mask);
-      const float d = static_cast<float>(p.D), r = rsqrtf(ss / d + p.eps), m = gx * r / d;
+      for (int e = 0; e < 2 * E; e += 2) {
+        ffma2(s0, s1, f[e], f[e + 1], f[e], f[e + 1], s0, s1);
+        fmul2(gw[e], gw[e + 1], g[e], g[e + 1], w[e], w[e + 1]);
+        ffma2(t0, t1, gw[e], gw[e + 1], f[e], f[e + 1], t0, t1);
+      }
+      const float ss = group_sum<LANES>(s0 + s1, mask), gx = group_sum<LANES>(t0 + t1, mask);
+      const float r = rsqrtf(ss * p.inv_D + p.eps), m = -gx * r * p.inv_D;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float nrm = f[e] * r;
-        dw[e] = fmaf(g[e], nrm, dw[e]);
-        g[e] = r * (g[e] * w[e] - nrm * m);
+      for (int e = 0; e < 2 * E; e += 2) {
+        float n0, n1, u0, u1;
+        fmul2(n0, n1, f[e], f[e + 1], r, r);
+        ffma2(dw[e], dw[e + 1], g[e], g[e + 1], n0, n1, dw[e], dw[e + 1]);
+        ffma2(u0, u1, n0, n1, m, m, gw[e], gw[e + 1]);
+        fmul2(g[e], g[e + 1], u0, u1, r, r);
       }
     }
     if (c.live) {
-      *reinterpret_cast<typename V::type*>(dx + (h0 + i) * p.D + c.a) = V::pack(g);
-      *reinterpret_cast<typename V::type*>(dx + (h0 + i) * p.D + c.b) = V::pack(g + 4);
+      Raw<T> o;
+      o.pack(g);
+      o.store(dx + (h0 + i) * p.D + c.a);
+      o.pack(g + E);
+      o.store(dx + (h0 + i) * p.D + c.b);
     }
   }
 }
 
-template <typename T, int LANES>
+// A block walks tokens blockIdx.x, + gridDim.x, .. (grid.y: shares of the heads
+// when there are few tokens), summing dw in registers; its sums go to
+// partial[block][q, k][D], added by weight_kernel in block order (no atomics:
+// the same bits every run).
+template <typename T, int LANES, bool INTER>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const Params p) {
+  constexpr int N = 2;  // x and dy of two heads in flight
+  constexpr int kGroups = kThreads / LANES;
   pdl_launch_dependents();
   const Group<LANES> g;
-  const Place c = place_of(g.lane, p);
-  __shared__ float sums[kThreads / LANES][LANES * 8 + 4];
+  const Place<INTER> c(g.lane, p);
+  __shared__ float sums[kGroups][LANES * 2 * E + 4];
   pdl_wait();
-  constexpr int kGroups = kThreads / LANES;
   for (int is_k = 0; is_k < 2; ++is_k) {
     const Stream& s = is_k ? p.k : p.q;
-    float w[8], dw[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float w[2 * E], dw[2 * E];
+#pragma unroll
+    for (int e = 0; e < 2 * E; ++e) dw[e] = 0.0f;
     load_weight<T>(s.weight, p.weight_f32, c, w);
-    // grid.y shares the heads; without a norm nothing is summed
     for (int64_t t = g.token; t < s.tokens; t += static_cast<int64_t>(gridDim.x) * kGroups) {
-      float cs[4], sn[4];
-      load_turn(p, c, g.lane, s.positions ? s.positions[t] : t % s.period, cs, sn);
-      for (int h = 0; h < s.heads; h += kGradHeads)
-        backward_heads<T, LANES>(static_cast<const T*>(s.x) + t * s.stride, static_cast<const T*>(s.dy) + t * s.dy_stride,
-                                 static_cast<T*>(s.y) + t * s.heads * p.D, s.heads, h, p, c, w, s.weight != nullptr, cs,
-                                 sn, g.mask, dw);
+      float cs[E], sn[E];
+      load_turn(p, c, g.lane, s.positions ? s.positions[t] : static_cast<int>(t) % s.period, cs, sn);
+      for (int h = blockIdx.y * N; h < s.heads; h += gridDim.y * N)
+        backward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + t * s.stride,
+                                              static_cast<const T*>(s.dy) + t * s.dy_stride,
+                                              static_cast<T*>(s.y) + t * s.heads * p.D, s.heads, h, p, c, w,
+                                              s.weight != nullptr, cs, sn, g.mask, dw);
     }
     if (!s.weight) continue;  // the same for the whole grid
     const int row = threadIdx.x / LANES;
     __syncthreads();
     if (c.live) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[row][c.a + e] = dw[e], sums[row][c.b + e] = dw[4 + e];
+      for (int e = 0; e < E; ++e) sums[row][c.a + e] = dw[e], sums[row][c.b + e] = dw[E + e];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < p.D; i += kThreads) {
       float a = 0.0f;
-#pragma unroll
+#pragma unroll 8
       for (int r = 0; r < kGroups; ++r) a += sums[r][i];
-      p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + is_k) * p.D + i] = a;
+      p.partial[((static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * 2 + is_k) * p.D + i] = a;
     }
   }
 }

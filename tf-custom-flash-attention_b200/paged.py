@@ -26,38 +26,45 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import InvalidArgumentError, _check
-from .rotary import _check_features, _dtype_of, _ptr, _rows, _same, _table, _weights
+from .ops import InvalidArgumentError
+from .rotary import _CUDA_MSG, _check_features, _dtype_of, _launch, _ptr, _rows, _same, _table, _weights
 
 
-def _check_batch(page_table, kv_len, q_start, ref: torch.Tensor):
+def _check_batch(page_table, kv_len, q_start, device):
+    """(N, M) of a batch's index tensors."""
     for x, name, dim in ((page_table, "page_table", 2), (kv_len, "kv_len", 1), (q_start, "q_start", 1)):
         if x.dtype != torch.int32 or x.dim() != dim or not x.is_contiguous():
             raise InvalidArgumentError(f"{name} must be a contiguous int32 tensor of rank {dim}")
-        _same(x, ref, name)
-    N = kv_len.shape[0]
-    if page_table.shape[0] != N or q_start.shape[0] != N + 1:
+        if x.device != device:
+            _same(x, device, name)
+    N, M = page_table.shape
+    if kv_len.shape[0] != N or q_start.shape[0] != N + 1:
         raise InvalidArgumentError("page_table must be [N, M], kv_len [N] and q_start [N+1]")
-    return N
+    return N, M
 
 
-def _check_pools(k_pages, v_pages, ref: torch.Tensor):
+def _check_pools(k_pages, v_pages, dtype, device):
+    """(pages, page size, H_kv, D, D_v) of the pools."""
     for x, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         if x.dim() != 4 or not x.is_contiguous():
             raise InvalidArgumentError(f"{name} must be a contiguous [pages, page_size, H_kv, D] tensor")
-        if x.dtype != ref.dtype:
+        if x.dtype != dtype:
             raise InvalidArgumentError("all floating-point inputs must share dtype T")
-        _same(x, ref, name)
+        if x.device != device:
+            _same(x, device, name)
         if x.data_ptr() % 16:
             raise InvalidArgumentError(f"{name} must start at a multiple of 16 bytes")
-    if k_pages.shape[:3] != v_pages.shape[:3]:
-        raise InvalidArgumentError("k_pages and v_pages must have the same pages, page size and heads")
     P, page, H_kv, D = k_pages.shape
+    vP, vpage, vH, D_v = v_pages.shape
+    if vP != P or vpage != page or vH != H_kv:
+        raise InvalidArgumentError("k_pages and v_pages must have the same pages, page size and heads")
+    if P < 1 or H_kv < 1:
+        raise InvalidArgumentError("the pools must hold at least one page and one head")
     if page < 16 or page > 65536 or page & (page - 1):
         raise InvalidArgumentError(f"page_size must be a power of two from 16 to 65536, got {page}")
     _check_features(D)
-    _check_features(v_pages.shape[3], "value feature size")
-    return P, page, H_kv, D, v_pages.shape[3]
+    _check_features(D_v, "value feature size")
+    return P, page, H_kv, D, D_v
 
 
 def _check_tokens(x: torch.Tensor, name: str, T: int, D: int, H, dtype):
@@ -80,37 +87,36 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     dt = _dtype_of(k)
     if k.dim() != 3:
         raise InvalidArgumentError(f"k must be [T, H_kv, D] but is rank {k.dim()}")
-    _same(k, k, "k")
-    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, k)
-    N = _check_batch(page_table, kv_len, q_start, k)
-    T = k.shape[0]
-    _check_tokens(k, "k", T, D, H_kv, k.dtype)
-    _check_tokens(v, "v", T, D_v, H_kv, k.dtype)
-    _same(v, k, "v")
+    if not k.is_cuda:
+        raise InvalidArgumentError(_CUDA_MSG)
+    dtype, device, T = k.dtype, k.device, k.shape[0]
+    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, dtype, device)
+    N, M = _check_batch(page_table, kv_len, q_start, device)
+    _check_tokens(k, "k", T, D, H_kv, dtype)
+    _check_tokens(v, "v", T, D_v, H_kv, dtype)
+    _same(v, device, "v")
     if q is not None:
-        _check_tokens(q, "q", T, D, None, k.dtype)
-        _same(q, k, "q")
+        _check_tokens(q, "q", T, D, None, dtype)
+        _same(q, device, "q")
     elif q_weight is not None:
         raise InvalidArgumentError("q_weight without q")
-    qw, kw, wdt = _weights(q_weight, k_weight, k, D)
-    table, max_pos, rot = _table(table, k, D)
+    qw, kw, wdt = _weights(q_weight, k_weight, dtype, device, D)
+    table, max_pos, rot = _table(table, device, D)
     align = 8 if dt == _lib.F16 else 4
-    kx, ks = _rows(k, align)
-    vx, vs = _rows(v, align)
+    kx, ks = _rows(k, H_kv * D, align)
+    vx, vs = _rows(v, H_kv * D_v, align)
     q_out, qx, qs, H_q = None, None, 0, 0
     if q is not None:
-        qx, qs = _rows(q, align)
         H_q = q.shape[1]
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    with torch.cuda.device(k.device):
-        st = torch.cuda.current_stream().cuda_stream
-        rc = _lib.lib().sdpa_b200_paged_append(
-            dt, _ptr(qx), qs, kx.data_ptr(), ks, vx.data_ptr(), vs, T, H_q, H_kv, D, D_v, _ptr(qw), _ptr(kw), wdt,
-            float(eps), _ptr(table), max_pos, rot, int(bool(interleaved)), _ptr(q_out), k_pages.data_ptr(),
-            v_pages.data_ptr(), P, page, page_table.data_ptr(), page_table.shape[1], kv_len.data_ptr(),
-            q_start.data_ptr(), N, st)
-    _check(rc)
+        qx, qs = _rows(q, H_q * D, align)
+        q_out = torch.empty(q.shape, dtype=dtype, device=device)
+    _launch(device, _lib.lib().sdpa_b200_paged_append, dt, _ptr(qx), qs, kx.data_ptr(), ks, vx.data_ptr(), vs, T, H_q, H_kv, D,
+            D_v, _ptr(qw), _ptr(kw), wdt, float(eps), _ptr(table), max_pos, rot, int(bool(interleaved)), _ptr(q_out),
+            k_pages.data_ptr(), v_pages.data_ptr(), P, page, page_table.data_ptr(), M, kv_len.data_ptr(), q_start.data_ptr(), N)
     return q_out
+
+
+_workspace_bytes: dict = {}  # of paged_sdpa, by what the query depends on
 
 
 def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -129,35 +135,41 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     dt = _dtype_of(q)
     if q.dim() != 3:
         raise InvalidArgumentError(f"q must be [T, H_q, D] but is rank {q.dim()}")
-    _same(q, q, "q")
-    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, q)
-    N = _check_batch(page_table, kv_len, q_start, q)
-    T, H_q = q.shape[0], q.shape[1]
-    _check_tokens(q, "q", T, D, None, q.dtype)
-    if H_kv < 1 or H_q < 1 or H_q % H_kv:
+    if not q.is_cuda:
+        raise InvalidArgumentError(_CUDA_MSG)
+    dtype, device = q.dtype, q.device
+    T, H_q, q_D = q.shape
+    P, page, H_kv, D, D_v = _check_pools(k_pages, v_pages, dtype, device)
+    N, M = _check_batch(page_table, kv_len, q_start, device)
+    if q_D != D:
+        raise InvalidArgumentError(f"q must be [{T}, H, {D}], got {list(q.shape)}")
+    if H_q < 1 or H_q % H_kv:
         raise InvalidArgumentError("H_q must be a multiple of H_kv")
     if out is None:
-        o = torch.empty((T, H_q, D_v), dtype=q.dtype, device=q.device)
-        stats = torch.empty((T, H_q), dtype=torch.float32, device=q.device)
+        o = torch.empty((T, H_q, D_v), dtype=dtype, device=device)
+        stats = torch.empty((T, H_q), dtype=torch.float32, device=device)
     else:
         o, stats = out
-        if tuple(o.shape) != (T, H_q, D_v) or o.dtype != q.dtype or not o.is_contiguous():
-            raise InvalidArgumentError("out[0] must be a contiguous [T, H_q, D_v] tensor of dtype T")
+        if tuple(o.shape) != (T, H_q, D_v) or o.dtype != dtype or not o.is_contiguous() or o.data_ptr() % 16:
+            raise InvalidArgumentError("out[0] must be a contiguous [T, H_q, D_v] tensor of dtype T, 16-byte aligned")
         if tuple(stats.shape) != (T, H_q) or stats.dtype != torch.float32 or not stats.is_contiguous():
             raise InvalidArgumentError("out[1] must be a contiguous float32 [T, H_q] tensor")
-        _same(o, q, "out[0]")
-        _same(stats, q, "out[1]")
+        _same(o, device, "out[0]")
+        _same(stats, device, "out[1]")
     if T == 0 or N == 0:
         return o, stats
-    qx, qs = _rows(q, 8 if dt == _lib.F16 else 4)
+    qx, qs = _rows(q, H_q * D, 8 if dt == _lib.F16 else 4)
     L = _lib.lib()
-    with torch.cuda.device(q.device):
-        ws_bytes = L.sdpa_b200_paged_workspace_bytes(dt, T, N, H_q, H_kv, D, D_v)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-        st = torch.cuda.current_stream().cuda_stream
-        rc = L.sdpa_b200_paged_sdpa(
-            dt, qx.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(), stats.data_ptr(), T, H_q, H_kv, D,
-            D_v, P, page, page_table.data_ptr(), page_table.shape[1], kv_len.data_ptr(), q_start.data_ptr(), N,
-            float(scale), int(bool(causal_mask)), ws.data_ptr(), ws_bytes, st)
-    _check(rc)
+    key = (dt, T, N, H_q, H_kv, D, D_v, device.index)
+    ws_bytes = _workspace_bytes.get(key)
+    if ws_bytes is None:
+        with torch.cuda.device(device):
+            ws_bytes = L.sdpa_b200_paged_workspace_bytes(dt, T, N, H_q, H_kv, D, D_v)
+        if len(_workspace_bytes) >= 4096:
+            _workspace_bytes.clear()
+        _workspace_bytes[key] = ws_bytes
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    _launch(device, L.sdpa_b200_paged_sdpa, dt, qx.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(),
+            stats.data_ptr(), T, H_q, H_kv, D, D_v, P, page, page_table.data_ptr(), M, kv_len.data_ptr(), q_start.data_ptr(), N,
+            float(scale), int(bool(causal_mask)), ws.data_ptr(), ws_bytes)
     return o, stats

@@ -14,6 +14,8 @@ layer takes its queries and keys as they are (mha.py:103-129).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -35,6 +37,9 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, dev
     return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
+_CUDA_MSG = "sdpa_b200 runs on CUDA tensors only (no CPU kernel is registered)"
+
+
 def _dtype_of(x: torch.Tensor) -> int:
     dt = _DTYPES.get(x.dtype)
     if dt is None:
@@ -42,35 +47,39 @@ def _dtype_of(x: torch.Tensor) -> int:
     return dt
 
 
-def _same(x: torch.Tensor, ref: torch.Tensor, name: str):
-    if not x.is_cuda:
-        raise InvalidArgumentError("sdpa_b200 runs on CUDA tensors only (no CPU kernel is registered)")
-    if x.device != ref.device:
-        raise InvalidArgumentError(f"{name} must be on {ref.device} like the other inputs, got {x.device}")
+def _same(x: torch.Tensor, device, name: str):
+    if x.device != device:
+        if not x.is_cuda:
+            raise InvalidArgumentError(_CUDA_MSG)
+        raise InvalidArgumentError(f"{name} must be on {device} like the other inputs, got {x.device}")
 
 
-def _rows(x: torch.Tensor, align: int):
-    """x [..., H, D] as (tensor, elements between tokens), its last two axes dense; copies only where they are not."""
-    H, D = x.shape[-2], x.shape[-1]
+def _launch(device, entry, *args):
+    """Calls a C ABI entry on `device` with its current stream as the last argument."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _rows(x: torch.Tensor, row: int, align: int):
+    """x [..., H, D] as (tensor, elements between tokens), its last two axes (`row` elements) dense; copies only
+    where they are not."""
     if not x.is_contiguous():
+        H, D = x.shape[-2], x.shape[-1]
         try:
             y = x.view(-1, H, D)
         except RuntimeError:
             y = None
         if (y is not None and (D == 1 or y.stride(2) == 1) and (H == 1 or y.stride(1) == D) and y.data_ptr() % 16 == 0
-                and (y.shape[0] == 1 or (y.stride(0) >= H * D and y.stride(0) % align == 0))):
-            return y, (H * D if y.shape[0] == 1 else y.stride(0))
+                and (y.shape[0] == 1 or (y.stride(0) >= row and y.stride(0) % align == 0))):
+            return y, (row if y.shape[0] == 1 else y.stride(0))
         x = x.contiguous()
     if x.data_ptr() % 16:
         x = x.clone()
-    return x, H * D
-
-
-def _check_heads(x: torch.Tensor, name: str, D: int):
-    if x.dim() < 3:
-        raise InvalidArgumentError(f"{name} must be [..., S, H, D] but is rank {x.dim()}")
-    if x.shape[-1] != D:
-        raise InvalidArgumentError("K feature size mismatch")
+    return x, row
 
 
 def _check_features(D: int, what: str = "feature size"):
@@ -80,48 +89,52 @@ def _check_features(D: int, what: str = "feature size"):
         raise InvalidArgumentError(f"{what} must be a multiple of 8, got {D}")
 
 
-def _weights(q_weight, k_weight, q: torch.Tensor, D: int):
+def _weight(w, dtype, device, D: int):
+    if w is None:
+        return None
+    if w.dim() != 1 or w.shape[0] != D:
+        raise InvalidArgumentError(f"a norm weight must be [{D}], got {list(w.shape)}")
+    if w.dtype != dtype and w.dtype != torch.float32:
+        raise InvalidArgumentError("norm weights must have dtype T or float32")
+    _same(w, device, "a norm weight")
+    return w.contiguous()
+
+
+def _weights(q_weight, k_weight, dtype, device, D: int):
     """(q weight, k weight, dtype code) of the norms."""
-    code = _DTYPES[q.dtype]
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    for w in given:
-        if w.dim() != 1 or w.shape[0] != D:
-            raise InvalidArgumentError(f"a norm weight must be [{D}], got {list(w.shape)}")
-        if w.dtype not in (q.dtype, torch.float32):
-            raise InvalidArgumentError("norm weights must have dtype T or float32")
-        _same(w, q, "a norm weight")
-    if given:
-        if given[0].dtype != given[-1].dtype:
-            raise InvalidArgumentError("q_weight and k_weight must share a dtype")
-        code = _DTYPES[given[0].dtype]
-    return (None if q_weight is None else q_weight.contiguous(), None if k_weight is None else k_weight.contiguous(), code)
+    q_weight, k_weight = _weight(q_weight, dtype, device, D), _weight(k_weight, dtype, device, D)
+    if q_weight is None:
+        return None, k_weight, _DTYPES[dtype if k_weight is None else k_weight.dtype]
+    if k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise InvalidArgumentError("q_weight and k_weight must share a dtype")
+    return q_weight, k_weight, _DTYPES[q_weight.dtype]
 
 
-def _table(table, q: torch.Tensor, D: int):
+def _table(table, device, D: int):
     """(table, positions it holds, rotated features)."""
     if table is None:
         return None, 0, 0
     if table.dim() != 2 or table.dtype != torch.float32:
         raise InvalidArgumentError("table must be float32 [max_positions, rotary_dim]")
-    rot = table.shape[1]
+    positions, rot = table.shape
     if rot < 8 or rot % 8 or rot > D:
         raise InvalidArgumentError(f"rotary_dim must be a multiple of 8 no larger than the feature size, got {rot}")
-    if table.shape[0] < 1:
+    if positions < 1:
         raise InvalidArgumentError("table must hold at least one position")
-    _same(table, q, "table")
+    _same(table, device, "table")
     if not table.is_contiguous() or table.data_ptr() % 16:
         table = table.clone(memory_format=torch.contiguous_format)
-    return table, table.shape[0], rot
+    return table, positions, rot
 
 
-def _positions(pos, x: torch.Tensor, name: str):
+def _positions(pos, lead, device, name: str):
     if pos is None:
         return None
     if pos.dtype.is_floating_point or pos.dtype == torch.bool:
         raise InvalidArgumentError(f"{name} must be integers")
-    if tuple(pos.shape) != tuple(x.shape[:-2]):
-        raise InvalidArgumentError(f"{name} must be {list(x.shape[:-2])}, got {list(pos.shape)}")
-    _same(pos, x, name)
+    if pos.shape != lead:
+        raise InvalidArgumentError(f"{name} must be {list(lead)}, got {list(pos.shape)}")
+    _same(pos, device, name)
     return pos.to(torch.int32).contiguous()
 
 
@@ -129,30 +142,42 @@ def _ptr(x):
     return None if x is None else x.data_ptr()
 
 
-def _prepare(q, k, q_weight, k_weight, table, q_positions, k_positions):
-    D = q.shape[-1] if q.dim() else 0
-    _check_heads(q, "q", D)
-    _check_heads(k, "k", D)
-    _check_features(D)
-    dt = _dtype_of(q)
-    if k.dtype != q.dtype:
-        raise InvalidArgumentError("all floating-point inputs must share dtype T")
-    _same(q, q, "q")
-    _same(k, q, "k")
-    qw, kw, wdt = _weights(q_weight, k_weight, q, D)
-    table, max_pos, rot = _table(table, q, D)
-    if q_positions is not None and k_positions is None and q.shape[:-2] == k.shape[:-2]:
-        k_positions = q_positions
-    qp = _positions(q_positions, q, "q_positions")
-    kp = qp if k_positions is q_positions else _positions(k_positions, k, "k_positions")
-    return D, dt, qw, kw, wdt, table, max_pos, rot, qp, kp
+class _Call:
+    """The checked arguments of one call, in the C ABI's terms."""
 
+    __slots__ = ("dt", "device", "D", "q", "k", "qs", "ks", "q_lead", "k_lead", "q_tokens", "k_tokens", "H_q", "H_k", "align",
+                 "qw", "kw", "rest", "qp", "kp")
 
-def _tokens(x: torch.Tensor) -> int:
-    n = 1
-    for s in x.shape[:-2]:
-        n *= s
-    return n
+    def __init__(self, q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved):
+        qshape, kshape = q.shape, k.shape
+        for shape, name in ((qshape, "q"), (kshape, "k")):
+            if len(shape) < 3:
+                raise InvalidArgumentError(f"{name} must be [..., S, H, D] but is rank {len(shape)}")
+        self.D = D = qshape[-1]
+        if kshape[-1] != D:
+            raise InvalidArgumentError("K feature size mismatch")
+        _check_features(D)
+        self.dt = _dtype_of(q)
+        if k.dtype != q.dtype:
+            raise InvalidArgumentError("all floating-point inputs must share dtype T")
+        if not q.is_cuda:
+            raise InvalidArgumentError(_CUDA_MSG)
+        self.device = device = q.device
+        _same(k, device, "k")
+        self.qw, self.kw, wdt = _weights(q_weight, k_weight, q.dtype, device, D)
+        table, max_pos, rot = _table(table, device, D)
+        # (the tensors are kept until the launch: a copy made here must outlive it)
+        self.rest = (table, wdt, float(eps), None if table is None else table.data_ptr(), max_pos, rot, int(bool(interleaved)))
+        self.q_lead, self.k_lead = qshape[:-2], kshape[:-2]
+        if q_positions is not None and k_positions is None and self.q_lead == self.k_lead:
+            k_positions = q_positions
+        self.qp = _positions(q_positions, self.q_lead, device, "q_positions")
+        self.kp = self.qp if k_positions is q_positions else _positions(k_positions, self.k_lead, device, "k_positions")
+        self.H_q, self.H_k = qshape[-2], kshape[-2]
+        self.q_tokens, self.k_tokens = math.prod(self.q_lead), math.prod(self.k_lead)
+        self.align = 8 if self.dt == _lib.F16 else 4
+        self.q, self.qs = _rows(q, self.H_q * D, self.align)
+        self.k, self.ks = _rows(k, self.H_k * D, self.align)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight=None, k_weight=None, table=None, q_positions=None,
@@ -165,19 +190,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight=None, k_weight=None,
     to 0 .. S_k-1.  A position the table does not hold is clamped to its ends and
     raises bit 1 of ``device_status``.  Inputs may be strided along S (slices of
     a fused projection); outputs are contiguous."""
-    D, dt, qw, kw, wdt, table, max_pos, rot, qp, kp = _prepare(q, k, q_weight, k_weight, table, q_positions, k_positions)
-    align = 8 if dt == _lib.F16 else 4
-    qx, qs = _rows(q, align)
-    kx, ks = _rows(k, align)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with torch.cuda.device(q.device):
-        st = torch.cuda.current_stream().cuda_stream
-        rc = _lib.lib().sdpa_b200_qk_norm_rope(
-            dt, qx.data_ptr(), _tokens(q), q.shape[-2], qs, _ptr(qp), max(q.shape[-3], 1), kx.data_ptr(), _tokens(k),
-            k.shape[-2], ks, _ptr(kp), max(k.shape[-3], 1), D, _ptr(qw), _ptr(kw), wdt, float(eps), _ptr(table), max_pos,
-            rot, int(bool(interleaved)), q_out.data_ptr(), k_out.data_ptr(), st)
-    _check(rc)
+    c = _Call(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=c.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=c.device)
+    _launch(c.device, _lib.lib().sdpa_b200_qk_norm_rope, c.dt, c.q.data_ptr(), c.q_tokens, c.H_q, c.qs, _ptr(c.qp),
+            c.q_lead[-1] or 1, c.k.data_ptr(), c.k_tokens, c.H_k, c.ks, _ptr(c.kp), c.k_lead[-1] or 1, c.D, _ptr(c.qw),
+            _ptr(c.kw), *c.rest[1:], q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -188,31 +206,23 @@ def qk_norm_rope_grad(q: torch.Tensor, k: torch.Tensor, dq_out: torch.Tensor, dk
 
     Weight gradients have the weights' dtype (None without a weight); they are
     summed in fp32 in a fixed order, so every run gives the same bits."""
-    D, dt, qw, kw, wdt, table, max_pos, rot, qp, kp = _prepare(q, k, q_weight, k_weight, table, q_positions, k_positions)
+    c = _Call(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
     for x, ref, name in ((dq_out, q, "dq_out"), (dk_out, k, "dk_out")):
         if x.shape != ref.shape or x.dtype != ref.dtype:
             raise InvalidArgumentError(f"{name} must have the shape and dtype of its input")
-        _same(x, ref, name)
-    align = 8 if dt == _lib.F16 else 4
-    qx, qs = _rows(q, align)
-    kx, ks = _rows(k, align)
-    gq, gqs = _rows(dq_out, align)
-    gk, gks = _rows(dk_out, align)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    dqw = None if qw is None else torch.empty_like(qw)
-    dkw = None if kw is None else torch.empty_like(kw)
-    L = _lib.lib()
+        _same(x, c.device, name)
+    gq, gqs = _rows(dq_out, c.H_q * c.D, c.align)
+    gk, gks = _rows(dk_out, c.H_k * c.D, c.align)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=c.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=c.device)
+    dqw = None if c.qw is None else torch.empty_like(c.qw)
+    dkw = None if c.kw is None else torch.empty_like(c.kw)
     ws_bytes, ws = 0, None
-    if qw is not None or kw is not None:
-        ws_bytes = L.sdpa_b200_qk_norm_rope_bwd_workspace_bytes(D)
-        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        st = torch.cuda.current_stream().cuda_stream
-        rc = L.sdpa_b200_qk_norm_rope_bwd(
-            dt, qx.data_ptr(), gq.data_ptr(), _tokens(q), q.shape[-2], qs, gqs, _ptr(qp), max(q.shape[-3], 1),
-            kx.data_ptr(), gk.data_ptr(), _tokens(k), k.shape[-2], ks, gks, _ptr(kp), max(k.shape[-3], 1), D, _ptr(qw),
-            _ptr(kw), wdt, float(eps), _ptr(table), max_pos, rot, int(bool(interleaved)), dq.data_ptr(), dk.data_ptr(),
-            _ptr(dqw), _ptr(dkw), _ptr(ws), ws_bytes, st)
-    _check(rc)
+    if dqw is not None or dkw is not None:
+        ws_bytes = _lib.lib().sdpa_b200_qk_norm_rope_bwd_workspace_bytes(c.D)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=c.device)
+    _launch(c.device, _lib.lib().sdpa_b200_qk_norm_rope_bwd, c.dt, c.q.data_ptr(), gq.data_ptr(), c.q_tokens, c.H_q, c.qs, gqs,
+            _ptr(c.qp), c.q_lead[-1] or 1, c.k.data_ptr(), gk.data_ptr(), c.k_tokens, c.H_k, c.ks, gks, _ptr(c.kp),
+            c.k_lead[-1] or 1, c.D, _ptr(c.qw), _ptr(c.kw), *c.rest[1:], dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw),
+            _ptr(ws), ws_bytes)
     return dq, dk, dqw, dkw
