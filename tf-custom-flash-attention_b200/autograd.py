@@ -94,5 +94,9 @@ class QKNormRopeFunction(torch.autograd.Function):
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, table=None, q_positions=None, k_positions=None, eps: float = 1e-6,
                  interleaved: bool = False):
-    """Differentiable ``rotary.qk_norm_rope``: gradients for q, k and the norm weights."""
+    """Differentiable ``rotary.qk_norm_rope``: gradients for q, k and the norm weights.
+
+    A step captured into a CUDA graph needs leaves of which no eager autograd
+    graph is alive (torch would join the capture with the stream of the old one
+    and invalidate it)."""
     return QKNormRopeFunction.apply(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)

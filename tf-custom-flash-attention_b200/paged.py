@@ -173,3 +173,74 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
             stats.data_ptr(), T, H_q, H_kv, D, D_v, P, page, page_table.data_ptr(), M, kv_len.data_ptr(), q_start.data_ptr(), N,
             float(scale), int(bool(causal_mask)), ws.data_ptr(), ws_bytes)
     return o, stats
+
+
+class PagedBatch:
+    """The index tensors of one serving step (``PagedCache.batch``): page_table, kv_len, q_start, and its tokens."""
+
+    __slots__ = ("page_table", "kv_len", "q_start", "tokens")
+
+    def __init__(self, page_table, kv_len, q_start, tokens: int):
+        self.page_table, self.kv_len, self.q_start, self.tokens = page_table, kv_len, q_start, tokens
+
+
+class PagedCache:
+    """Pools of one attention layer and the page accounting of its sequences.
+
+    ``batch([(sequence, new_tokens), ..])`` reserves room for the new tokens
+    (sequence ids are any hashable; a new id starts an empty sequence) and
+    returns the step's ``PagedBatch``; ``append`` and ``attend`` run on it;
+    ``free`` gives a sequence's pages back.  Several layers with equal lengths can
+    share one cache object's accounting by passing its batches to their own
+    pools (``paged_append`` / ``paged_sdpa``)."""
+
+    def __init__(self, pages: int, page_size: int, heads: int, head_dim: int, value_dim=None, dtype=torch.float16, device=None):
+        dev = torch.device(device or "cuda")
+        self.k_pages = torch.zeros(pages, page_size, heads, head_dim, dtype=dtype, device=dev)
+        self.v_pages = torch.zeros(pages, page_size, heads, head_dim if value_dim is None else value_dim, dtype=dtype, device=dev)
+        self.page_size = page_size
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages: dict = {}   # sequence -> its pages in order
+        self._length: dict = {}  # sequence -> cached tokens
+
+    def length(self, sequence) -> int:
+        """Tokens cached (or reserved) for a sequence; 0 for one that is not held."""
+        return self._length.get(sequence, 0)
+
+    def batch(self, new_tokens) -> PagedBatch:
+        """Reserves `count` further tokens for each (sequence, count); nothing is reserved if the pages do not suffice."""
+        new_tokens = [(s, int(c)) for s, c in new_tokens]
+        seen = {s for s, _ in new_tokens}
+        if len(seen) != len(new_tokens):
+            raise InvalidArgumentError("a sequence may appear once in a batch")
+        if any(c < 0 for _, c in new_tokens):
+            raise InvalidArgumentError("token counts must not be negative")
+        need = {s: -(-(self.length(s) + c) // self.page_size) - len(self._pages.get(s, ())) for s, c in new_tokens}
+        if sum(need.values()) > len(self._free):
+            raise InvalidArgumentError(f"the cache has {len(self._free)} free pages, the batch needs {sum(need.values())}")
+        start, rows, lengths = [0], [], []
+        for s, c in new_tokens:
+            pages = self._pages.setdefault(s, [])
+            pages.extend(self._free.pop() for _ in range(need[s]))
+            self._length[s] = self.length(s) + c
+            rows.append(pages)
+            lengths.append(self._length[s])
+            start.append(start[-1] + c)
+        width = max([1, *map(len, rows)])
+        index = torch.tensor([x for r in rows for x in (*r, *[-1] * (width - len(r)))] + lengths + start, dtype=torch.int32)
+        index = index.to(self.k_pages.device)  # one copy for the three
+        n = len(rows)
+        table, kv_len, q_start = index.split([n * width, n, n + 1])
+        return PagedBatch(table.view(n, width), kv_len, q_start, start[-1])
+
+    def free(self, sequence):
+        self._free.extend(reversed(self._pages.pop(sequence, [])))
+        self._length.pop(sequence, None)
+
+    def append(self, k, v, batch: PagedBatch, **kw):
+        """``paged_append`` into this cache's pools."""
+        return paged_append(k, v, self.k_pages, self.v_pages, batch.page_table, batch.kv_len, batch.q_start, **kw)
+
+    def attend(self, q, batch: PagedBatch, **kw):
+        """``paged_sdpa`` over this cache's pools."""
+        return paged_sdpa(q, self.k_pages, self.v_pages, batch.page_table, batch.kv_len, batch.q_start, **kw)
