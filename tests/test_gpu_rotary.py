@@ -237,3 +237,31 @@ def test_same_bits_every_run_on_two_streams_and_in_a_graph():
     torch.cuda.synchronize()
     for o in (*outs, captured):
         assert all(torch.equal(a, b) for a, b in zip(o, ref))
+
+
+@pytest.mark.parametrize("dtype,shape,hq,hk,d,rot,inter", [
+    (torch.float16, (3, 6500), 3, 1, 128, 128, False),   # a group walks several tokens: the loads run ahead
+    (torch.float16, (1, 40000), 1, 2, 40, 24, True),
+    (torch.float32, (2, 9700), 3, 2, 64, 32, False),
+])
+def test_long_inputs(dtype, shape, hq, hk, d, rot, inter):
+    """Forward and backward over more tokens than the backward's groups."""
+    case = (dtype, shape, hq, hk, d, rot, inter, True, True, torch.float32, True)
+    q, k, qw, kw, table, pos, where, _ = make(case, 4)
+    for x, w, y in zip((q, k), (qw, kw), fa.qk_norm_rope(q, k, qw, kw, table, pos, eps=1e-5, interleaved=inter)):
+        ref = turn64(norm64(x, w, 1e-5), table, where, inter)
+        close(y, ref, x.dtype, ref.abs().amax(-1, keepdim=True))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    dys = [torch.randn(x.shape, generator=g, device="cuda").to(dtype) for x in (q, k)]
+    grads = fa.qk_norm_rope_grad(q, k, *dys, qw, kw, table, pos, eps=1e-5, interleaved=inter)
+    for x, w, dy, dx, dw in ((q, qw, dys[0], grads[0], grads[2]), (k, kw, dys[1], grads[1], grads[3])):
+        gr = turn64(dy.double(), table, where, inter, -1.0)
+        x64 = x.double()
+        r = torch.rsqrt((x64 * x64).mean(-1, keepdim=True) + 1e-5)
+        n, gw = x64 * r, gr * w.double()
+        size = r * (gw.abs().amax(-1, keepdim=True) + n.abs().amax(-1, keepdim=True) * (gw * n).abs().mean(-1, keepdim=True))
+        close(dx, r * (gw - n * (gw * n).mean(-1, keepdim=True)), dtype, size)
+        terms = (gr * n).flatten(0, -2)
+        # a lane adds under 64 rows here, the tree behind it 48 more: see test_backward
+        assert ((dw.double() - terms.sum(0)).abs() <= 128 * 2.0 ** -24 * terms.abs().sum(0) + 2.0 ** -24 * terms.sum(0).abs()).all()
+    assert fa.device_status() == 0

@@ -18,11 +18,13 @@ int shares(int64_t tokens, int lanes, int units) {
 }
 
 template <typename Kernel>
-int launch_grid(Kernel kern, int64_t gx, int gy, int threads, cudaStream_t st, const rotary::Params& p, int* launches) {
+int launch_grid(Kernel kern, int64_t gx, int gy, int threads, size_t smem, cudaStream_t st, const rotary::Params& p,
+                int* launches) {
   if (gx <= 0 || gx > 0x7fffffffLL || gy > 65535) return SDPA_B200_EINVAL;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -46,20 +48,29 @@ int launch_t(rotary::Params p, int what, cudaStream_t st, int* launches) {
     const int64_t gx = std::min<int64_t>(rotary::kGradBlocks, std::max<int64_t>(1, (tokens + kGroups - 1) / kGroups));
     const int gy = static_cast<int>(std::min<int64_t>(std::max({1, p.q.heads / 4, p.k.heads / 4}), rotary::kGradBlocks / gx));
     p.blocks = static_cast<int>(gx) * gy;
-    if (int r = launch_grid(rotary::backward_kernel<T, LANES, INTER>, gx, gy, rotary::kThreads, st, p, launches)) return r;
+    if (tokens > static_cast<int64_t>(rotary::kGradBlocks) * kGroups) {  // more than one a group: see backward_kernel
+      static std::atomic<uint64_t> attr_done{0};
+      constexpr size_t kRing = rotary::kStages<T> * rotary::kStageBytes<T>;
+      auto kern = rotary::backward_kernel<T, LANES, INTER, true>;
+      if (cudaError_t e = ensure_smem(kern, kRing, attr_done)) return cuda_failure("shared-memory attribute", e);
+      if (int r = launch_grid(kern, gx, gy, rotary::kThreads, kRing, st, p, launches)) return r;
+    } else {
+      auto kern = rotary::backward_kernel<T, LANES, INTER, false>;
+      if (int r = launch_grid(kern, gx, gy, rotary::kThreads, 0, st, p, launches)) return r;
+    }
     if (!p.dw_q && !p.dw_k) return SDPA_B200_OK;
-    return launch_grid(rotary::weight_kernel<T>, (p.D + 31) / 32, 2, 1024, st, p, launches);
+    return launch_grid(rotary::weight_kernel<T>, (p.D + 31) / 32, 2, 1024, 0, st, p, launches);
   }
   const int heads = rotary::units_of(p.q.heads, N) + rotary::units_of(p.k.heads, N);
   if (what == kForward) {
     const int64_t tokens = std::max(p.q.tokens, p.k.tokens);
     return launch_grid(rotary::forward_kernel<T, LANES, INTER>, (tokens + kGroups - 1) / kGroups,
-                       shares(tokens, LANES, heads), rotary::kThreads, st, p, launches);
+                       shares(tokens, LANES, heads), rotary::kThreads, 0, st, p, launches);
   }
   const int nv = p.k.heads * p.D_v / static_cast<int>(16 / sizeof(T));
   return launch_grid(rotary::append_kernel<T, LANES, INTER>, (p.view.tokens + kGroups - 1) / kGroups,
                      shares(p.view.tokens, LANES, heads + rotary::units_of(nv, LANES * rotary::kCopyWords)), rotary::kThreads,
-                     st, p, launches);
+                     0, st, p, launches);
 }
 
 // Eight features a lane, a power of two of lanes a head row.

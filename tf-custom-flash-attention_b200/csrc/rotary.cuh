@@ -13,9 +13,10 @@
 // pairs 8j..), weights, cosines and sines are multiplied once a token, and the
 // products go in packed pairs (f32x2).  A group walks the heads of one token,
 // four at a time with all their loads ahead of the arithmetic.  32768 tokens x
-// 32 heads x 128 in fp16: forward 108 us (537 MB, 5.0 TB/s), backward 200 us (805 MB,
-// 4.0 TB/s); with the weights and the turn apart 120 and 215 us; sixteen features a
-// lane (16-byte loads, fewer instructions, but over 110 registers) 118 and 205 us.
+// 32 heads x 128 in fp16: forward 99 us (537 MB, 5.4 TB/s), backward 151 us (805 MB,
+// 5.3 TB/s).  Measured worse: the weights and the turn applied apart (120 us forward);
+// sixteen features a lane, with 16-byte loads and fewer instructions but over 110
+// registers (118 us); the forward's loads through a ring as the backward's (99 us).
 // All arithmetic is fp32, rounded to T once, at the store.
 #pragma once
 #include "common.cuh"
@@ -182,17 +183,12 @@ __device__ __forceinline__ float group_sum(float x, unsigned mask) {
   return x;
 }
 
-// Heads [h0, h0 + N) of one token's row: norm, rotation, store.
+// Norm, rotation and store of heads [h0, h0 + N) of one token, as loaded.
 template <typename T, int LANES, bool INTER, int N>
-__device__ __forceinline__ void forward_heads(const T* x, T* y, int heads, int h0, const Params& p,
+__device__ __forceinline__ void forward_heads(const Raw<T>* ra, const Raw<T>* rb, T* y, int heads, int h0, const Params& p,
                                               const Place<INTER>& c, const Turn& w, bool norm, unsigned mask) {
   using P = Place<INTER>;
-  Raw<T> ra[N], rb[N];
-  const T *xa = x + h0 * p.D + c.a, *xb = x + h0 * p.D + c.b;
   T *ya = y + h0 * p.D + c.a, *yb = y + h0 * p.D + c.b;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (c.live && h0 + i < heads) ra[i].load(xa + i * p.D), rb[i].load(xb + i * p.D);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (h0 + i >= heads) break;  // the same for every lane of the group
@@ -229,7 +225,44 @@ __device__ __forceinline__ void forward_heads(const T* x, T* y, int heads, int h
   }
 }
 
-constexpr int kHeadsAhead = 4;  // heads a group has in flight
+// A lane's ring in shared memory: words of one run of E features, kThreads
+// apart, written by the lane's own cp.async and read by itself (no barrier).
+template <typename T>
+struct Ring {
+  static constexpr int kWord = E * sizeof(T);  // 8 or 16 bytes
+  uint8_t* base;
+  __device__ __forceinline__ explicit Ring(uint8_t* smem) : base(smem + threadIdx.x * kWord) {}
+  __device__ __forceinline__ void copy(int word, const T* src) {
+    const uint32_t dst = smem_u32(base + word * (kThreads * kWord));
+    if (kWord == 8)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    else
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  }
+  __device__ __forceinline__ Raw<T> read(int word) const {
+    Raw<T> r;
+    if (kWord == 8) {
+      const uint2 x = *reinterpret_cast<const uint2*>(base + word * (kThreads * kWord));
+      r.w[0] = x.x, r.w[1] = x.y;
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(base + word * (kThreads * kWord));
+      r.w[0] = x.x, r.w[1] = x.y, r.w[kWord / 4 - 2] = x.z, r.w[kWord / 4 - 1] = x.w;
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  template <int N>
+  static __device__ __forceinline__ void wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  }
+};
+
+constexpr int kHeadsAhead = 4;  // heads a group takes at a time
+// Stages of the backward's ring, each x and dy of two heads: eight words a lane.
+template <typename T>
+constexpr int kStages = sizeof(T) == 2 ? 4 : 2;
+template <typename T>
+constexpr int kStageBytes = 8 * kThreads * E * static_cast<int>(sizeof(T));
 // Blocks an SM (fp16: 64 registers a thread; fp32 holds twice the loads).  At
 // 64 the append kernel spills some addresses and gains all the same: 38 us
 // against 46 for 5251 tokens x 48 heads x 128.
@@ -270,6 +303,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) forward_kernel(const Par
     const bool is_k = u >= uq;
     const Stream& s = is_k ? p.k : p.q;
     if (g.token >= s.tokens) continue;
+    const int h0 = (is_k ? u - uq : u) * N;
+    const T* x = static_cast<const T*>(s.x) + g.token * s.stride + h0 * p.D;
+    Raw<T> ra[N], rb[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c.live && h0 + i < s.heads) ra[i].load(x + i * p.D + c.a), rb[i].load(x + i * p.D + c.b);
     const int64_t pos = s.positions ? s.positions[g.token] : static_cast<int>(g.token) % s.period;
     if (kind != (is_k ? 1 : 0) || pos != at) {
       float cs[E], sn[E], w[2 * E];
@@ -279,9 +318,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) forward_kernel(const Par
       kind = is_k ? 1 : 0;
       at = pos;
     }
-    forward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + g.token * s.stride,
-                                         static_cast<T*>(s.y) + g.token * s.heads * p.D, s.heads, (is_k ? u - uq : u) * N,
-                                         p, c, turn, s.weight != nullptr, g.mask);
+    forward_heads<T, LANES, INTER, N>(ra, rb, static_cast<T*>(s.y) + g.token * s.heads * p.D, s.heads, h0, p, c, turn,
+                                      s.weight != nullptr, g.mask);
   }
 }
 
@@ -338,31 +376,30 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) append_kernel(const Para
       kind = is_k ? 1 : 0;
     }
     T* y = is_k ? static_cast<T*>(p.k_pages) + slot * s.heads * p.D : static_cast<T*>(s.y) + g.token * s.heads * p.D;
-    forward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + g.token * s.stride, y, s.heads,
-                                         (is_k ? u - uq : u) * N, p, c, turn, s.weight != nullptr, g.mask);
+    const int h0 = (is_k ? u - uq : u) * N;
+    const T* x = static_cast<const T*>(s.x) + g.token * s.stride + h0 * p.D;
+    Raw<T> ra[N], rb[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c.live && h0 + i < s.heads) ra[i].load(x + i * p.D + c.a), rb[i].load(x + i * p.D + c.b);
+    forward_heads<T, LANES, INTER, N>(ra, rb, y, s.heads, h0, p, c, turn, s.weight != nullptr, g.mask);
   }
 }
 
-// Backward, heads [h0, h0 + N) of one token's row: dx, and dw summed.
+// Backward of heads [h0, h0 + N) of one token, as loaded (x: a, b, dy: a, b of
+// each head): dx, and dw summed.
 template <typename T, int LANES, bool INTER, int N>
-__device__ __forceinline__ void backward_heads(const T* x, const T* dy, T* dx, int heads, int h0, const Params& p,
+__device__ __forceinline__ void backward_heads(const Raw<T> (&in)[N][4], T* dx, int heads, int h0, const Params& p,
                                                const Place<INTER>& c, const float* w, bool norm, const float* cs,
                                                const float* sn, unsigned mask, float* dw) {
   using P = Place<INTER>;
-  Raw<T> xa[N], xb[N], ga[N], gb[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (c.live && h0 + i < heads) {
-      if (norm) xa[i].load(x + (h0 + i) * p.D + c.a), xb[i].load(x + (h0 + i) * p.D + c.b);
-      ga[i].load(dy + (h0 + i) * p.D + c.a), gb[i].load(dy + (h0 + i) * p.D + c.b);
-    }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (h0 + i >= heads) break;
     float d[2 * E], g[2 * E];
 #pragma unroll
     for (int e = 0; e < 2 * E; ++e) d[e] = 0.0f;
-    if (c.live) ga[i].unpack(d), gb[i].unpack(d + E);
+    if (c.live) in[i][2].unpack(d), in[i][3].unpack(d + E);
 #pragma unroll
     for (int e = 0; e < E; e += 2) {  // g = R^T dy
       const float a0 = d[P::first(e)], a1 = d[P::first(e + 1)], b0 = d[P::second(e)], b1 = d[P::second(e + 1)];
@@ -376,7 +413,7 @@ __device__ __forceinline__ void backward_heads(const T* x, const T* dy, T* dx, i
       float f[2 * E], gw[2 * E];
 #pragma unroll
       for (int e = 0; e < 2 * E; ++e) f[e] = 0.0f;
-      if (c.live) xa[i].unpack(f), xb[i].unpack(f + E);
+      if (c.live) in[i][0].unpack(f), in[i][1].unpack(f + E);
       // both sums at once: mean(g w n) = r * mean(g w x)
       float s0 = 0.0f, s1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
 #pragma unroll
@@ -408,31 +445,81 @@ __device__ __forceinline__ void backward_heads(const T* x, const T* dy, T* dx, i
 
 // A block walks tokens blockIdx.x, + gridDim.x, .. (grid.y: shares of the heads
 // when there are few tokens), summing dw in registers; its sums go to
-// partial[block][q, k][D], added by weight_kernel in block order (no atomics:
-// the same bits every run).
-template <typename T, int LANES, bool INTER>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Params p) {
-  constexpr int N = 2;  // x and dy of two heads in flight
+// partial[block][q, k][D], added by weight_kernel in block order (no atomics: the
+// same bits every run).  RING: the loads run kStages - 1 head pairs ahead, through
+// shared memory (at its registers two blocks an SM fit, whose own loads are too few
+// in flight: 151 us against 191 for 32768 tokens x 32 heads x 128 fp16).  Worth it
+// where a group walks several tokens; with one the ring only adds a step (4099 tokens
+// x 16 heads x 64 fp32: 22 us against 16).
+template <typename T, int LANES, bool INTER, bool RING>
+__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Params p) {
+  constexpr int N = 2, ST = kStages<T>;  // x and dy of two heads a stage
   constexpr int kGroups = kThreads / LANES;
+  extern __shared__ __align__(16) uint8_t smem[];
   pdl_launch_dependents();
   const Group<LANES> g;
   const Place<INTER> c(g.lane, p);
+  Ring<T> ring(smem);
   __shared__ float sums[kGroups][LANES * 2 * E + 4];
   pdl_wait();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   for (int is_k = 0; is_k < 2; ++is_k) {
     const Stream& s = is_k ? p.k : p.q;
+    const bool norm = s.weight != nullptr;
     float w[2 * E], dw[2 * E];
 #pragma unroll
     for (int e = 0; e < 2 * E; ++e) dw[e] = 0.0f;
     load_weight<T>(s.weight, p.weight_f32, c, w);
-    for (int64_t t = g.token; t < s.tokens; t += static_cast<int64_t>(gridDim.x) * kGroups) {
+    int64_t t_in = g.token;  // the walk of the loads
+    int h_in = blockIdx.y * N, stage_in = 0, stage = 0;
+    auto load = [&]() {
+      if (t_in < s.tokens && h_in < s.heads) {
+        if (c.live) {
+          const T* x = static_cast<const T*>(s.x) + t_in * s.stride + h_in * p.D;
+          const T* dy = static_cast<const T*>(s.dy) + t_in * s.dy_stride + h_in * p.D;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (h_in + i < s.heads) {
+              const int word = (stage_in * N + i) * 4;
+              if (norm) ring.copy(word, x + i * p.D + c.a), ring.copy(word + 1, x + i * p.D + c.b);
+              ring.copy(word + 2, dy + i * p.D + c.a), ring.copy(word + 3, dy + i * p.D + c.b);
+            }
+        }
+        if ((h_in += gridDim.y * N) >= s.heads) h_in = blockIdx.y * N, t_in += step;
+        if (++stage_in == ST) stage_in = 0;
+      }
+      ring.commit();
+    };
+    if (RING) {
+#pragma unroll
+      for (int i = 0; i < ST - 1; ++i) load();
+    }
+    for (int64_t t = g.token; t < s.tokens; t += step) {
       float cs[E], sn[E];
       load_turn(p, c, g.lane, s.positions ? s.positions[t] : static_cast<int>(t) % s.period, cs, sn);
-      for (int h = blockIdx.y * N; h < s.heads; h += gridDim.y * N)
-        backward_heads<T, LANES, INTER, N>(static_cast<const T*>(s.x) + t * s.stride,
-                                              static_cast<const T*>(s.dy) + t * s.dy_stride,
-                                              static_cast<T*>(s.y) + t * s.heads * p.D, s.heads, h, p, c, w,
-                                              s.weight != nullptr, cs, sn, g.mask, dw);
+      for (int h = blockIdx.y * N; h < s.heads; h += gridDim.y * N) {
+        Raw<T> in[N][4];
+        if (RING) {
+          ring.template wait<ST - 2>();
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) in[i][k] = ring.read((stage * N + i) * 4 + k);
+          if (++stage == ST) stage = 0;
+          load();  // into the stage that the last pair has left
+        } else {
+          const T* x = static_cast<const T*>(s.x) + t * s.stride + h * p.D;
+          const T* dy = static_cast<const T*>(s.dy) + t * s.dy_stride + h * p.D;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (c.live && h + i < s.heads) {
+              if (norm) in[i][0].load(x + i * p.D + c.a), in[i][1].load(x + i * p.D + c.b);
+              in[i][2].load(dy + i * p.D + c.a), in[i][3].load(dy + i * p.D + c.b);
+            }
+        }
+        backward_heads<T, LANES, INTER, N>(in, static_cast<T*>(s.y) + t * s.heads * p.D, s.heads, h, p, c, w, norm, cs, sn,
+                                           g.mask, dw);
+      }
     }
     if (!s.weight) continue;  // the same for the whole grid
     const int row = threadIdx.x / LANES;
