@@ -263,11 +263,13 @@ template <typename T>
 constexpr int kStages = sizeof(T) == 2 ? 4 : 2;
 template <typename T>
 constexpr int kStageBytes = 8 * kThreads * E * static_cast<int>(sizeof(T));
-// Blocks an SM (fp16: 64 registers a thread; fp32 holds twice the loads).  At
-// 64 the append kernel spills some addresses and gains all the same: 38 us
-// against 46 for 5251 tokens x 48 heads x 128.
+// Blocks an SM (fp32 holds twice the loads): forward (fp16: 64 registers a
+// thread), and append, whose addresses would spill there (5251 tokens x 48 heads
+// x 128 fp16: 35 us against 37 with four blocks, 46 with two).
 template <typename T>
 constexpr int kBlocks = sizeof(T) == 2 ? 4 : 3;
+template <typename T>
+constexpr int kAppendBlocks = sizeof(T) == 2 ? 3 : 2;
 // Head groups of a stream.
 __host__ __device__ __forceinline__ int units_of(int heads, int ahead) { return (heads + ahead - 1) / ahead; }
 
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) forward_kernel(const Par
 // the table, and on pages outside the pool are not written.
 constexpr int kCopyWords = 4;  // 16-byte words of the values a lane has in flight
 template <typename T, int LANES, bool INTER>
-__global__ void __launch_bounds__(kThreads, kBlocks<T>) append_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kAppendBlocks<T>) append_kernel(const Params p) {
   constexpr int N = kHeadsAhead;
   pdl_launch_dependents();
   const Group<LANES> g;
@@ -337,8 +339,28 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) append_kernel(const Para
   pdl_wait();
   const int uq = units_of(p.q.heads, N), uk = units_of(p.k.heads, N);
   const int nv = p.k.heads * p.D_v / kVec;  // a token's values in 16-byte words, contiguous on both sides
-  const int uv = units_of(nv, LANES * kCopyWords);
+  const int uv = units_of(nv, LANES * kCopyWords), units = uq + uk + uv;
   if (g.token >= p.view.tokens) return;
+  Raw<T> ra[N], rb[N];
+  uint4 words[kCopyWords];
+  auto load = [&](int u) {
+    if (u >= uq + uk) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.x) + g.token * p.v.stride);
+      const int i0 = (u - uq - uk) * LANES * kCopyWords + g.lane;
+#pragma unroll
+      for (int i = 0; i < kCopyWords; ++i)
+        if (i0 + i * LANES < nv) words[i] = __ldg(src + i0 + i * LANES);
+    } else {
+      const Stream& s = u >= uq ? p.k : p.q;
+      const int h0 = (u >= uq ? u - uq : u) * N;
+      const T* x = static_cast<const T*>(s.x) + g.token * s.stride + h0 * p.D;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c.live && h0 + i < s.heads) ra[i].load(x + i * p.D + c.a), rb[i].load(x + i * p.D + c.b);
+    }
+  };
+  int u = blockIdx.y;
+  load(u);  // on its way while the token's place is looked up (four dependent reads)
   const int n = seq_of_token<LANES>(p.view, static_cast<int>(g.token), g.mask, g.lane);
   if (n < 0) return;
   const int64_t held = p.view.kv_len[n];
@@ -351,38 +373,30 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) append_kernel(const Para
   load_turn(p, c, g.lane, pos, cs, sn);
   Turn turn;
   int kind = -1;  // the stream that `turn` is of
-  for (int u = blockIdx.y; u < uq + uk + uv; u += gridDim.y) {
+  while (true) {
     if (u >= uq + uk) {
-      if (page < 0) continue;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.x) + g.token * p.v.stride);
       uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.v_pages) + slot * p.k.heads * p.D_v);
       const int i0 = (u - uq - uk) * LANES * kCopyWords + g.lane;
-      uint4 r[kCopyWords];
 #pragma unroll
       for (int i = 0; i < kCopyWords; ++i)
-        if (i0 + i * LANES < nv) r[i] = __ldg(src + i0 + i * LANES);
-#pragma unroll
-      for (int i = 0; i < kCopyWords; ++i)
-        if (i0 + i * LANES < nv) dst[i0 + i * LANES] = r[i];
-      continue;
+        if (page >= 0 && i0 + i * LANES < nv) dst[i0 + i * LANES] = words[i];
+    } else {
+      const bool is_k = u >= uq;
+      const Stream& s = is_k ? p.k : p.q;
+      if (!is_k || page >= 0) {
+        if (kind != (is_k ? 1 : 0)) {
+          float w[2 * E];
+          load_weight<T>(s.weight, p.weight_f32, c, w);
+          turn.set<INTER>(w, cs, sn);
+          kind = is_k ? 1 : 0;
+        }
+        T* y = is_k ? static_cast<T*>(p.k_pages) + slot * s.heads * p.D : static_cast<T*>(s.y) + g.token * s.heads * p.D;
+        forward_heads<T, LANES, INTER, N>(ra, rb, y, s.heads, (is_k ? u - uq : u) * N, p, c, turn, s.weight != nullptr,
+                                          g.mask);
+      }
     }
-    const bool is_k = u >= uq;
-    if (is_k && page < 0) continue;
-    const Stream& s = is_k ? p.k : p.q;
-    if (kind != (is_k ? 1 : 0)) {
-      float w[2 * E];
-      load_weight<T>(s.weight, p.weight_f32, c, w);
-      turn.set<INTER>(w, cs, sn);
-      kind = is_k ? 1 : 0;
-    }
-    T* y = is_k ? static_cast<T*>(p.k_pages) + slot * s.heads * p.D : static_cast<T*>(s.y) + g.token * s.heads * p.D;
-    const int h0 = (is_k ? u - uq : u) * N;
-    const T* x = static_cast<const T*>(s.x) + g.token * s.stride + h0 * p.D;
-    Raw<T> ra[N], rb[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c.live && h0 + i < s.heads) ra[i].load(x + i * p.D + c.a), rb[i].load(x + i * p.D + c.b);
-    forward_heads<T, LANES, INTER, N>(ra, rb, y, s.heads, h0, p, c, turn, s.weight != nullptr, g.mask);
+    if ((u += gridDim.y) >= units) break;
+    load(u);
   }
 }
 

@@ -109,7 +109,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if q is not None:
         H_q = q.shape[1]
         qx, qs = _rows(q, H_q * D, align)
-        q_out = torch.empty(q.shape, dtype=dtype, device=device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _launch(device, _lib.lib().sdpa_b200_paged_append, dt, _ptr(qx), qs, kx.data_ptr(), ks, vx.data_ptr(), vs, T, H_q, H_kv, D,
             D_v, _ptr(qw), _ptr(kw), wdt, float(eps), _ptr(table), max_pos, rot, int(bool(interleaved)), _ptr(q_out),
             k_pages.data_ptr(), v_pages.data_ptr(), P, page, page_table.data_ptr(), M, kv_len.data_ptr(), q_start.data_ptr(), N)
@@ -146,7 +146,8 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     if H_q < 1 or H_q % H_kv:
         raise InvalidArgumentError("H_q must be a multiple of H_kv")
     if out is None:
-        o = torch.empty((T, H_q, D_v), dtype=dtype, device=device)
+        o = torch.empty_like(q, memory_format=torch.contiguous_format) if D_v == D else torch.empty(
+            (T, H_q, D_v), dtype=dtype, device=device)
         stats = torch.empty((T, H_q), dtype=torch.float32, device=device)
     else:
         o, stats = out

@@ -191,8 +191,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight=None, k_weight=None,
     raises bit 1 of ``device_status``.  Inputs may be strided along S (slices of
     a fused projection); outputs are contiguous."""
     c = _Call(q, k, q_weight, k_weight, table, q_positions, k_positions, eps, interleaved)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=c.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=c.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     _launch(c.device, _lib.lib().sdpa_b200_qk_norm_rope, c.dt, c.q.data_ptr(), c.q_tokens, c.H_q, c.qs, _ptr(c.qp),
             c.q_lead[-1] or 1, c.k.data_ptr(), c.k_tokens, c.H_k, c.ks, _ptr(c.kp), c.k_lead[-1] or 1, c.D, _ptr(c.qw),
             _ptr(c.kw), *c.rest[1:], q_out.data_ptr(), k_out.data_ptr())
@@ -213,8 +213,8 @@ def qk_norm_rope_grad(q: torch.Tensor, k: torch.Tensor, dq_out: torch.Tensor, dk
         _same(x, c.device, name)
     gq, gqs = _rows(dq_out, c.H_q * c.D, c.align)
     gk, gks = _rows(dk_out, c.H_k * c.D, c.align)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=c.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=c.device)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     dqw = None if c.qw is None else torch.empty_like(c.qw)
     dkw = None if c.kw is None else torch.empty_like(c.kw)
     ws_bytes, ws = 0, None
