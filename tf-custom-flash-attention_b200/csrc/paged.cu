@@ -12,26 +12,24 @@ namespace {
 
 int bucket_of(int64_t D, int64_t D_v) { return std::max(D, D_v) <= 64 ? 64 : 128; }
 
-// The kernel a call takes.  The lengths are on the device: the rule goes by the
-// call's tokens and sequences.  fp16: the tcgen05 kernel (groups of up to 128
-// heads, what its row tiles hold) where a sequence may have more packed rows
-// (new tokens x heads of a group) than a group of warps of the few-row kernel
-// takes together, 16 to 64; it reads the keys of single tokens among the chunks
-// at the rate of HBM as well (0.65 us a tile of 64 keys and SM: 7 TB/s).  The
-// few-row kernel for the rest: a token a sequence (32 x 8192 keys: 75 us
-// against 105 on the other), drafts that cannot be longer, and fp32, with its
-// row tiles from the mean of packed rows.
+// The kernel a call takes.  The lengths are on the device, so the rule goes by
+// the call's tokens and sequences alone.  fp16: the few-row kernel for a token a
+// sequence, or so few more that none can have over 16 packed rows (new tokens x
+// heads of a group); the tcgen05 kernel for the rest with groups of up to 128
+// heads, what its row tiles hold.  It serves single tokens among chunks as well
+// (few-row and tcgen05 kernel, us: 16 x 32768 keys x 4 heads 181 and 178; 32
+// ragged to 8192 keys x 8 heads 57 and 90; 64 x 1000 keys, 8 / 16 / 32 rows, 58 / 63
+// / 84 and 75 / 77 / 79; one token of 32 heads to a KV head, 8 x 4096 keys, 62 and
+// 18), while a chunk in the few-row kernel reads its keys once every 16 rows.
+// fp32: the few-row kernel, its row tiles from the mean of packed rows.
 struct Plan {
   bool tc;
   int mt;  // row tiles of 16 of a group of warps
 };
 Plan plan_of(int dtype, int64_t tokens, int64_t seqs, int64_t group) {
-  if (dtype != SDPA_B200_F16 || group > 128) {
-    const int64_t mean = (tokens * group + seqs - 1) / seqs;
-    return {false, mean <= 16 ? 1 : mean <= 32 ? 2 : 4};
-  }
-  const int mt = group <= 16 ? 1 : group <= 32 ? 2 : 4;
-  return {group > 64 || (tokens > seqs && (tokens - seqs + 1) * group > 16 * mt), mt};
+  if (dtype == SDPA_B200_F16 && group <= 128) return {group > 16 || (tokens > seqs && (tokens - seqs + 1) * group > 16), 1};
+  const int64_t mean = (tokens * group + seqs - 1) / seqs;
+  return {false, mean <= 16 ? 1 : mean <= 32 ? 2 : 4};
 }
 
 // Workspace of the few-row kernel: [ranges][2][rows] sums, (max, sum) pairs, one record a range.

@@ -15,16 +15,18 @@
 // always inside one page) go to the warp's own ring of kStages blocks in shared
 // memory, 128-byte swizzled, so the matrix operands come out of it without
 // bank conflicts (ldmatrix; for fp32 values 16-byte loads, four output columns
-// a word), and no barrier of the CTA stands in the loop.  (Operands copied lane
-// by lane, with plain loads or cp.async, took 450 instructions a block of 16
-// keys and 196 / 243 us for 16 x 32768 keys x 4 heads; this takes about 170.)
+// a word), and no barrier of the CTA stands in the loop.  16 x 32768 keys x 4 heads x
+// 128 fp16 take 183 us (5.9 TB/s).  Operands copied lane by lane took 450
+// instructions a block of 16 keys instead of about 170, and 196 us (plain loads,
+// two blocks' worth of registers) or 243 us (cp.async).
 //
 // Work: every (sequence, KV head, row tile) item has ceil(held / 32) tiles of
 // 32 keys; the tiles of all items, in order, are cut into equal ranges, one a
 // warp (with more than 16 packed rows a sequence, one a group of 2 or 4 warps
 // with a row tile each), so long and short sequences load the device evenly.
 // An item that lies in one range is finished there; one that is cut leaves
-// partial sums, at most two a range, that merge_kernel joins.
+// partial sums, at most two a range, that merge_kernel joins (32 sequences of 64 to
+// 8192 keys x 8 heads x 128: 74 us, about 4 of them the merge).
 #pragma once
 #include "common.cuh"
 #include "fwd_tc.cuh"
@@ -35,6 +37,9 @@ namespace sdpa_b200 {
 namespace paged {
 
 constexpr int kTile = 32;       // keys of one unit of work
+constexpr int kLeast = 2;       // tiles of a range
+constexpr int kLong = 16;       // pieces behind the first from which an item is merged in kParts parts
+constexpr int kParts = 4;
 constexpr int kRows = 16;       // packed query rows of one matrix tile
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
@@ -55,7 +60,9 @@ struct Params {
   float* part_o;          // [ranges, 2, part_rows, part_cols] unnormalised sums
   float2* part_ml;        // [ranges, 2, part_rows] (max, sum), log2 units
   int4* part_item;        // [ranges] of the item cut at the range's end: (its sequence's first token, its first
-                          // packed row, its rows, KV head << 16 | ranges behind that hold the rest); 0 rows: none
+                          // packed row, its rows | part << 16, KV head << 16 | ranges behind its first that hold the
+                          // rest); 0 rows: none.  The range that an item begins in has part 0; of one with many
+                          // pieces the next ranges, inside it, have parts 1 to 3: four blocks merge its rows
   int part_ranges, part_rows, part_cols;
   // workspace of the chunk kernel: pieces of cut items
   float* tc_o;            // [slots, 256, DV]
@@ -224,7 +231,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   s_before[tid] = before + incl - mine;
   __syncthreads();
   const int64_t range = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(gridDim.x) * group;
-  const int64_t ranges = min(static_cast<int64_t>(gridDim.x) * S::kGroups, total);
+  // (fp16) fewer ranges where they would be short: one a warp scheduler, then kLeast tiles each
+  const int64_t most = min(static_cast<int64_t>(gridDim.x) * S::kGroups, total);
+  const int64_t ranges = HALF ? min(most, max(static_cast<int64_t>(4 * p.sms), total / kLeast)) : most;
   if (range >= ranges) {
     if (mt == 0 && lane == 0) p.part_item[range] = make_int4(0, 0, 0, 0);
     return;
@@ -497,10 +506,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
     const bool complete = tile0 == 0 && tiles == nt;
     const int slot = tile0 == 0 ? 1 : 0;  // 0: the item began before this range
-    if (!complete && slot == 1) {
-      const int64_t last = base + (item + 1) * nt;  // one past the item's last tile
-      record = make_int4(sl.begin, rtile * ROWS, min(ROWS, total_rows - rtile * ROWS),
-                         head << 16 | static_cast<int>((last * ranges - 1) / total - range));
+    if (!complete && w + tiles == w1) {  // cut at the range's end
+      const int64_t first_tile = base + item * nt;
+      const int64_t first = slot == 1 ? range : ((first_tile + 1) * ranges - 1) / total;  // the range it began in
+      const int more = static_cast<int>(((first_tile + nt) * ranges - 1) / total - first);
+      const int part = static_cast<int>(range - first);
+      if (part == 0 || (more >= kLong && part < kParts))
+        record = make_int4(sl.begin, rtile * ROWS, min(ROWS, total_rows - rtile * ROWS) | part << 16, head << 16 | more);
     }
     const float inv_a = complete ? row_scale(l_a) : 1.0f, inv_b = complete ? row_scale(l_b) : 1.0f;
     const int64_t oa = static_cast<int64_t>(sl.begin + ra / p.G) * p.H_q + head * p.G + ra % p.G;
@@ -573,18 +585,21 @@ __device__ __forceinline__ void join_pieces(const float* o, const float2* ml, in
   }
 }
 
+// Rows part, part + parts, .. of the item that began in range `range`.
 template <typename T>
-__device__ __forceinline__ void merge_range(const Params& p, int range, const int4& it, float4* s_acc, float2* s_ml) {
+__device__ __forceinline__ void merge_range(const Params& p, int range, int part, int parts, const int4& it,
+                                            float4* s_acc, float2* s_ml) {
   const int ROWS = p.part_rows, shift = p.part_cols == 64 ? 4 : 5;  // log2 of a row's float4 columns
-  const int rows = it.z, pieces = (it.w & 0xffff) + 1, head = it.w >> 16;
+  const int rows = (it.z - part + parts - 1) / parts, pieces = (it.w & 0xffff) + 1, head = it.w >> 16;
   // rows a round takes, and (where the item has fewer) shares of the pieces
   const int round = kMergeThreads >> shift, at_once = min(rows, round), shares = min(pieces, round / at_once);
   const int group = threadIdx.x >> shift, c = (threadIdx.x & ((1 << shift) - 1)) * 4;
   const int share = group / at_once, row_in = group - share * at_once;
   // piece 0 is slot 1 of its range, piece i slot 0 of range + i: rows (2 range + 1) ROWS, then 2 ROWS apart from + ROWS
   const int row0 = (range * 2 + 1) * ROWS;
-  for (int row = row_in; row - row_in < rows; row += at_once) {
-    const bool live = share < shares && row < rows;
+  for (int i_row = row_in; i_row - row_in < rows; i_row += at_once) {
+    const bool live = share < shares && i_row < rows;
+    const int row = part + i_row * parts;
     float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (live) {
@@ -624,8 +639,11 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const Params p) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) it[k] = i0 + k * stride < p.part_ranges ? p.part_item[i0 + k * stride] : make_int4(0, 0, 0, 0);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (it[k].z > 0) merge_range<T>(p, i0 + k * stride, it[k], s_acc, s_ml);
+    for (int k = 0; k < kAhead; ++k) {
+      const int part = it[k].z >> 16, parts = (it[k].w & 0xffff) >= kLong ? kParts : 1;
+      it[k].z &= 0xffff;
+      if (it[k].z > part) merge_range<T>(p, i0 + k * stride - part, part, parts, it[k], s_acc, s_ml);
+    }
   }
 }
 

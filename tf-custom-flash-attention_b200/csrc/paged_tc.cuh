@@ -165,10 +165,11 @@ struct Piece {
 __device__ __forceinline__ int pairs_of(const SeqLens& s, int tokens2) { return (s.count + tokens2 - 1) / tokens2; }
 __device__ __forceinline__ int tiles_of(const SeqLens& s) { return max(1, (s.held + kBN - 1) / kBN); }
 
-// Time of one of its items: a tile of 64 keys takes 1.15 us for a pair of row
-// tiles, 0.65 us where the tokens fill the first alone (D = 128).
+// Time of one of its items: a tile of 64 keys takes 1.10 us for a pair of row
+// tiles, 0.70 us where the tokens fill the first alone (D = 128; 0.90 and 0.66 us
+// for D = 64).
 __device__ __forceinline__ float cost_of(const SeqLens& s, int tokens2) {
-  return static_cast<float>(tiles_of(s)) * (s.count > tokens2 / 2 ? 9.0f : 5.0f);
+  return static_cast<float>(tiles_of(s)) * (s.count > tokens2 / 2 ? 9.0f : 6.0f);
 }
 constexpr float kStart = 54.0f;  // what a piece costs beside its tiles
 // Pieces of an item: its cost in quanta, rounded (a piece costs from 2/3 to 3/2
