@@ -119,6 +119,16 @@ ATTEND = [
     (torch.float16, [(200, 513)], 8, 8, 96, 72, 32, True),
     (torch.float16, [(200, 150), (170, 0), (140, 129)], 4, 2, 64, 128, 64, True),                       # chunks past their cache
     (torch.float16, [(520, 1032), (0, 5), (300, 300)], 2, 1, 128, 64, 512, True),
+    (torch.float16, [(70, 300)] * 40, 8, 8, 64, 64, 16, True),                                          # more items than SMs
+    (torch.float16, [(3, 100), (40, 41), (0, 3), (1, 700)] * 10, 8, 1, 128, 64, 32, True),              # over 32 sequences of chunks
+    (torch.float16, [(1, 1 + 37 * n % 500) for n in range(300)], 2, 1, 64, 64, 16, True),               # over 128 of single tokens
+    (torch.float16, [(4, 20000)], 4, 1, 64, 64, 64, True),                                              # many pieces
+    (torch.float16, [(1, 9000), (1, 5)], 33, 1, 64, 128, 128, True),                                    # wide groups
+    (torch.float16, [(3, 40), (1, 500)], 128, 1, 128, 128, 16, True),
+    (torch.float16, [(1, 50), (3, 400)], 130, 1, 64, 64, 16, True),
+    (torch.float16, [(2, 90)], 260, 2, 128, 128, 16, False),
+    (torch.float32, [(1, 1 + 53 * n % 300) for n in range(200)], 1, 1, 128, 128, 16, True),
+    (torch.float32, [(2, 15000)], 8, 1, 128, 128, 32, True),
     (torch.float32, [(1, 1), (1, 130)], 2, 2, 64, 64, 16, True),
     (torch.float32, [(4, 333), (1, 2000), (2, 1), (0, 9), (3, 0)], 6, 2, 128, 128, 32, True),
     (torch.float32, [(40, 200), (7, 64)], 8, 4, 40, 96, 16, False),
@@ -376,3 +386,19 @@ def test_host_mirror_refusals_on_the_device():
                             ((k, k, *rest), dict(q=k, q_weight=w, k_weight=w.half()), "share a dtype")]:
         with pytest.raises(E, match=words):
             fa.paged_append(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.float16, 1), (torch.float16, 200), (torch.float32, 3)])
+def test_a_nan_key_reaches_the_rows_that_see_it_and_no_others(dtype, new):
+    lens = [(new, 300), (new, 250)]
+    s = make(dtype, lens, 4, 2, 64, 64, 16, seed=4)
+    clean = fa.paged_sdpa(**s, scale=0.125)
+    for key in (297, 298, 299):  # of the first sequence, in the chunk's last columns or the token's own
+        k_pages = s["k_pages"].clone()
+        k_pages[s["page_table"][0, key // 16].item(), key % 16, 0] = float("nan")  # KV head 0: query heads 0 and 1
+        got = fa.paged_sdpa(**dict(s, k_pages=k_pages), scale=0.125)
+        sees = torch.zeros(2 * new, 4, dtype=torch.bool, device="cuda")
+        sees[max(0, key - (300 - new)):new, :2] = True
+        for a, b in zip(got, clean):
+            seen = sees if a.dim() == 2 else sees[..., None].expand_as(a)
+            assert a[seen].isnan().all() and torch.equal(a[~seen], b[~seen])

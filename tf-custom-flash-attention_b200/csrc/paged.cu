@@ -28,6 +28,7 @@ struct Plan {
 };
 Plan plan_of(int dtype, int64_t tokens, int64_t seqs, int64_t group) {
   if (dtype == SDPA_B200_F16 && group <= 128) return {group > 16 || (tokens > seqs && (tokens - seqs + 1) * group > 16), 1};
+  if (dtype == SDPA_B200_F16) return {false, 4};  // over 128 rows a token
   const int64_t mean = (tokens * group + seqs - 1) / seqs;
   return {false, mean <= 16 ? 1 : mean <= 32 ? 2 : 4};
 }
@@ -65,20 +66,16 @@ int launch_mma_t(const paged::Params& p, cudaStream_t st, int* launches) {
   return SDPA_B200_OK;
 }
 
-// f<T, DB, MT>(args) for the call's type, bucket and row tiles.
-#define SDPA_B200_PAGED_DISPATCH(F, dtype, db, mt, ...)                                             \
-  ((dtype) == SDPA_B200_F16                                                                         \
-       ? ((db) == 64 ? ((mt) == 1   ? F<__half, 64, 1>(__VA_ARGS__)                                 \
-                        : (mt) == 2 ? F<__half, 64, 2>(__VA_ARGS__)                                 \
-                                    : F<__half, 64, 4>(__VA_ARGS__))                                \
-                     : ((mt) == 1   ? F<__half, 128, 1>(__VA_ARGS__)                                \
-                        : (mt) == 2 ? F<__half, 128, 2>(__VA_ARGS__)                                \
-                                    : F<__half, 128, 4>(__VA_ARGS__)))                              \
-       : ((db) == 64 ? ((mt) == 1   ? F<float, 64, 1>(__VA_ARGS__)                                  \
-                        : (mt) == 2 ? F<float, 64, 2>(__VA_ARGS__)                                  \
-                                    : F<float, 64, 4>(__VA_ARGS__))                                 \
-                     : ((mt) == 1   ? F<float, 128, 1>(__VA_ARGS__)                                 \
-                        : (mt) == 2 ? F<float, 128, 2>(__VA_ARGS__)                                 \
+// F<T, DB, MT>(args) for the call's type, bucket and row tiles (fp16: 1 or 4).
+#define SDPA_B200_PAGED_DISPATCH(F, dtype, db, mt, ...)                                                   \
+  ((dtype) == SDPA_B200_F16                                                                               \
+       ? ((db) == 64 ? ((mt) == 1 ? F<__half, 64, 1>(__VA_ARGS__) : F<__half, 64, 4>(__VA_ARGS__))        \
+                     : ((mt) == 1 ? F<__half, 128, 1>(__VA_ARGS__) : F<__half, 128, 4>(__VA_ARGS__)))     \
+       : ((db) == 64 ? ((mt) == 1   ? F<float, 64, 1>(__VA_ARGS__)                                        \
+                        : (mt) == 2 ? F<float, 64, 2>(__VA_ARGS__)                                        \
+                                    : F<float, 64, 4>(__VA_ARGS__))                                       \
+                     : ((mt) == 1   ? F<float, 128, 1>(__VA_ARGS__)                                       \
+                        : (mt) == 2 ? F<float, 128, 2>(__VA_ARGS__)                                       \
                                     : F<float, 128, 4>(__VA_ARGS__))))
 
 size_t place_mma(const Plan& plan, int dtype, int db, paged::Params* p, uint8_t* w) {

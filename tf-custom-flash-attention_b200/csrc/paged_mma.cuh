@@ -85,12 +85,14 @@ __device__ __forceinline__ void mma_1688(float* d, const uint32_t* a, uint32_t b
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, both tf32 values: hi is x rounded to 11 bits (half away from
-// zero, by an integer add: the conversion instruction runs at a fraction of
-// the rate), lo the rounded rest.
+// x = hi + lo, both tf32 values, by Veltkamp's splitting: hi is x rounded to 11
+// bits, lo the rest (exact) cut to 11.  (The conversion instruction runs at a
+// fraction of the rate; adding half a step to the bits loses the NaN of all ones.)
 __device__ __forceinline__ void split_fast(float x, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+  const float c = __fmul_rn(x, 8193.0f);  // (each step rounded by itself, not fused)
+  const float h = __fsub_rn(c, __fsub_rn(c, x));
+  hi = __float_as_uint(h);
+  lo = __float_as_uint(__fsub_rn(x, h)) & 0xffffe000u;
 }
 __device__ __forceinline__ void split_fast(const uint4& x, uint4& hi, uint4& lo) {
   split_fast(__uint_as_float(x.x), hi.x, lo.x);
@@ -142,7 +144,7 @@ struct Shape {
 __device__ __forceinline__ float row_stats(float m, float l) {
   return (m == -INFINITY ? kNegInit : m * kLn2) + logf(l + kEps);
 }
-__device__ __forceinline__ float row_scale(float l) { return l > kEps ? 1.0f / l : 0.0f; }
+__device__ __forceinline__ float row_scale(float l) { return l <= kEps ? 0.0f : 1.0f / l; }  // (NaN stays)
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, float x, float y, float z, float w) {
   if (sizeof(T) == 2)

@@ -117,12 +117,13 @@ constexpr int kPolyOf8 = 2;  // of 8 pairs of scores, those whose exponentials g
 // to relieve the special function unit: x = n + f with n the nearest integer
 // (by the addition of 1.5 * 2^23), |f| <= 1/2, 2^f by a polynomial of degree 4
 // (least squares at Chebyshev nodes; off by 4e-6 at most, a sixtieth of the
-// rounding of P to fp16), n added to the exponent.  x below -126 gives 2^-126,
+// rounding of P to fp16), times 2^n.  x below -126 gives 2^-126,
 // which fp16 rounds to zero.
 __device__ __forceinline__ void exp2_pair(float& p0, float& p1, float r0, float r1, float s, float b) {
   float x0, x1, n0, n1, f0, f1;
   ffma2(x0, x1, r0, r1, s, s, b, b);
-  x0 = fmaxf(x0, -126.0f), x1 = fmaxf(x1, -126.0f);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));  // (a NaN score stays one)
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
   constexpr float kMagic = 12582912.0f;
   n0 = kMagic, n1 = kMagic;
   fadd2(n0, n1, x0, x1);
@@ -133,8 +134,8 @@ __device__ __forceinline__ void exp2_pair(float& p0, float& p1, float r0, float 
   ffma2(p0, p1, p0, p1, f0, f1, 0.240247443f, 0.240247443f);
   ffma2(p0, p1, p0, p1, f0, f1, 0.693121791f, 0.693121791f);
   ffma2(p0, p1, p0, p1, f0, f1, 0.999999285f, 0.999999285f);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+  fmul2(p0, p1, p0, p1, __uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u),
+        __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u));  // 2^n, exactly
 }
 
 // Whether three barriers have all passed (one vote: 75 cycles; three waits one
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t row = static_cast<int64_t>(sl.begin + tok) * p.H_q + w.head * p.G + r_in % p.G;
       const int64_t prow = static_cast<int64_t>(w.slot) * (2 * kBM) + t * kBM + r_in;
       const bool part = w.pieces > 1;
-      const float mul = part ? f : (l_true > kEps ? f / l_true : 0.0f);
+      const float mul = part ? f : (l_true <= kEps ? 0.0f : f / l_true);  // (NaN stays)
       if (active) {
         if (part)
           p.tc_ml[prow] = make_float2(m_run, l_true);
