@@ -388,6 +388,19 @@ def test_host_mirror_refusals_on_the_device():
             fa.paged_append(*args, **kw)
 
 
+def test_results_may_not_lie_over_the_queries():
+    s = make(torch.float16, [(1, 20), (2, 9)], 4, 2, 64, 64, 16)
+    pool = torch.zeros(6, 4, 64, device="cuda", dtype=torch.float16)
+    s["q"] = pool[:3]
+    stats = torch.empty(3, 4, device="cuda")
+    for out in (pool[:3], pool[2:5]):
+        with pytest.raises(fa.InvalidArgumentError, match="share memory"):
+            fa.paged_sdpa(**s, out=(out, stats))
+    with pytest.raises(fa.InvalidArgumentError, match="share memory"):
+        fa.paged_sdpa(**s, out=(pool[3:], pool.view(torch.float32).view(-1)[:12].view(3, 4)))
+    fa.paged_sdpa(**s, out=(pool[3:], stats))  # beside them
+
+
 @pytest.mark.parametrize("dtype,new", [(torch.float16, 1), (torch.float16, 200), (torch.float32, 3)])
 def test_a_nan_key_reaches_the_rows_that_see_it_and_no_others(dtype, new):
     lens = [(new, 300), (new, 250)]

@@ -193,6 +193,17 @@ def test_positions_outside_the_table_are_clamped_and_reported():
     assert torch.equal(y, ref) and fa.device_status() == 0
 
 
+@pytest.mark.parametrize("far", [2 ** 32 + 3, -(2 ** 32) + 3, 2 ** 31, 2 ** 62])
+def test_wide_positions_are_not_cut_to_a_row_of_the_table(far):
+    table = fa.rotary_table(8, 64)
+    q = torch.randn(1, 2, 2, 64, device="cuda")
+    fa.device_status()
+    y, _ = fa.qk_norm_rope(q, q, table=table, q_positions=torch.tensor([[1, far]], device="cuda"))
+    assert fa.device_status() == 2
+    ref, _ = fa.qk_norm_rope(q, q, table=table, q_positions=torch.tensor([[1, 0 if far < 0 else 7]], device="cuda"))
+    assert torch.equal(y, ref) and fa.device_status() == 0
+
+
 def test_far_positions():
     """Angles of 10^5 radians: the table is taken in float64."""
     table = fa.rotary_table(131072, 64, device="cuda")

@@ -125,3 +125,17 @@ def test_workspace_queries():
     assert L.sdpa_b200_paged_workspace_bytes(0, 4, 4, 8, 2, 64, 64) > 0
     assert L.sdpa_b200_qk_norm_rope_bwd_workspace_bytes(0) == 0
     assert L.sdpa_b200_qk_norm_rope_bwd_workspace_bytes(64) == 592 * 2 * 64 * 4
+
+
+@pytest.mark.parametrize("change", [dict(page_size=48), dict(page_size=8), dict(head_dim=12), dict(head_dim=136),
+                                    dict(value_dim=4), dict(pages=0), dict(heads=0), dict(dtype=torch.bfloat16)])
+def test_cache_refusals(change):
+    with pytest.raises(fa.InvalidArgumentError):
+        fa.PagedCache(**{**dict(pages=4, page_size=16, heads=2, head_dim=64, device="cpu"), **change})
+
+
+def test_shared_memory_is_seen():
+    x = torch.empty(64)
+    share = importlib.import_module("tf-custom-flash-attention_b200.paged")._share_bytes
+    assert share(x[:8], x[7:]) and share(x[::4], x[1:2]) and share(x, x)
+    assert not share(x[:8], x[8:]) and not share(x[:0], x) and not share(x[0:8:2], x[7:])

@@ -389,21 +389,36 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < KS; k += 2) {
-          uint32_t b[4], bl[4];  // two inner steps, two operands each
-          ldmatrix4(k_at + (k >> 2) * S::kBoxBytes + k_off + (((2 * (k & 3) + k_chunk) ^ sw) << 4), b);
+        for (int k = 0; k < KS; k += 4) {
+          uint32_t b[2][4], bl[2][4];  // twice two inner steps, two operands each
+          uint4 l[4];
+          float part[2][4];  // short sums on the tensor cores, joined in fp32
 #pragma unroll
-          for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(b[e]), b[e], bl[e]);
-          const uint4 l0 = q_lo[k * 32], l1 = q_lo[(k + 1) * 32];
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short sums on the tensor cores, joined in fp32
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&l0), b[0], b[1]);
-          mma_1688(part, reinterpret_cast<const uint32_t*>(&l1), b[2], b[3]);
-          mma_1688(part, qf[k], bl[0], bl[1]);
-          mma_1688(part, qf[k + 1], bl[2], bl[3]);
-          mma_1688(part, qf[k], b[0], b[1]);
-          mma_1688(part, qf[k + 1], b[2], b[3]);
+          for (int h = 0; h < 2; ++h) {
+            const int k2 = k + 2 * h;
+            ldmatrix4(k_at + (k2 >> 2) * S::kBoxBytes + k_off + (((2 * (k2 & 3) + k_chunk) ^ sw) << 4), b[h]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][e] += part[e];
+            for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(b[h][e]), b[h][e], bl[h][e]), part[h][e] = 0.0f;
+            l[2 * h] = q_lo[k2 * 32], l[2 * h + 1] = q_lo[(k2 + 1) * 32];
+          }
+          // two sums in turn: a product waits 21 cycles for the last one of its sum, 8 for another's
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              mma_1688(part[h], reinterpret_cast<const uint32_t*>(&l[2 * h + x]), b[h][2 * x], b[h][2 * x + 1]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma_1688(part[h], qf[k + 2 * h + x], bl[h][2 * x], bl[h][2 * x + 1]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma_1688(part[h], qf[k + 2 * h + x], b[h][2 * x], b[h][2 * x + 1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0][e] += part[h][e];
         }
       }
       // online softmax in log2 units
@@ -468,15 +483,17 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
           split_fast(*reinterpret_cast<const uint4*>(box + (2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4)), h1, l1);
           const uint32_t *xh0 = reinterpret_cast<const uint32_t*>(&h0), *xh1 = reinterpret_cast<const uint32_t*>(&h1);
           const uint32_t *xl0 = reinterpret_cast<const uint32_t*>(&l0), *xl1 = reinterpret_cast<const uint32_t*>(&l1);
+          float part[4][4] = {};  // (four sums in turn, as above)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_1688(part, pl, xh0[j], xh1[j]);
-            mma_1688(part, ph, xl0[j], xl1[j]);
-            mma_1688(part, ph, xh0[j], xh1[j]);
+          for (int j = 0; j < 4; ++j) mma_1688(part[j], pl, xh0[j], xh1[j]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * x + j][e] += part[e];
-          }
+          for (int j = 0; j < 4; ++j) mma_1688(part[j], ph, xl0[j], xl1[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_1688(part[j], ph, xh0[j], xh1[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * x + j][e] += part[j][e];
         }
       }
       __syncwarp();  // every lane has left the stage

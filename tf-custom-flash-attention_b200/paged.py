@@ -116,6 +116,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     return q_out
 
 
+def _share_bytes(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the stretches of memory from the first to the last element of two tensors meet (strides are not negative)."""
+    if not a.numel() or not b.numel():
+        return False
+    end = [x.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size() for x in (a, b)]
+    return a.data_ptr() < end[1] and b.data_ptr() < end[0]
+
+
 _workspace_bytes: dict = {}  # of paged_sdpa, by what the query depends on
 
 
@@ -124,11 +132,11 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     """Attention of new tokens q [T, H_q, D] over the cached keys of their sequences.
 
     Returns (output [T, H_q, D_v] T, stats [T, H_q] float32), stats as in
-    ``sdpa``: max + ln(sum + 1e-6) of the scaled scores.  H_q is a multiple of
+    ``sdpa``: max + ln(sum + 1e-6) of the scaled scores; no gradients.  H_q is a multiple of
     H_kv; query head h reads KV head h // (H_q / H_kv).  With ``causal_mask`` a
     token sees the keys up to its own position, else all kv_len of its sequence;
     one that sees none gets zeros and stats of -1e9.  ``out`` may pass
-    (output, stats) to write into; rows behind the last sequence keep what they
+    (output, stats) to write into, memory apart from q's; rows behind the last sequence keep what they
     held (and hold anything in a result allocated here).  A NaN or infinity
     cached behind a sequence's kv_len reaches nothing; one at a position that
     only later tokens of the same chunk see may reach the chunk's earlier rows."""
@@ -157,6 +165,9 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
             raise InvalidArgumentError("out[1] must be a contiguous float32 [T, H_q] tensor")
         _same(o, device, "out[0]")
         _same(stats, device, "out[1]")
+        for x, name in ((o, "out[0]"), (stats, "out[1]")):
+            if _share_bytes(x, q):
+                raise InvalidArgumentError(f"{name} must not share memory with q, whose rows other blocks still read")
     if T == 0 or N == 0:
         return o, stats
     qx, qs = _rows(q, H_q * D, 8 if dt == _lib.F16 else 4)
@@ -197,8 +208,10 @@ class PagedCache:
 
     def __init__(self, pages: int, page_size: int, heads: int, head_dim: int, value_dim=None, dtype=torch.float16, device=None):
         dev = torch.device(device or "cuda")
+        _dtype_of(torch.empty(0, dtype=dtype))  # fp16 or fp32
         self.k_pages = torch.zeros(pages, page_size, heads, head_dim, dtype=dtype, device=dev)
         self.v_pages = torch.zeros(pages, page_size, heads, head_dim if value_dim is None else value_dim, dtype=dtype, device=dev)
+        _check_pools(self.k_pages, self.v_pages, dtype, self.k_pages.device)
         self.page_size = page_size
         self._free = list(range(pages - 1, -1, -1))
         self._pages: dict = {}   # sequence -> its pages in order

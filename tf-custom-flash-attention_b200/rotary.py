@@ -130,12 +130,14 @@ def _table(table, device, D: int):
 def _positions(pos, lead, device, name: str):
     if pos is None:
         return None
-    if pos.dtype.is_floating_point or pos.dtype == torch.bool:
-        raise InvalidArgumentError(f"{name} must be integers")
+    if pos.dtype not in (torch.int32, torch.int64):
+        raise InvalidArgumentError(f"{name} must be int32 or int64")
     if pos.shape != lead:
         raise InvalidArgumentError(f"{name} must be {list(lead)}, got {list(pos.shape)}")
     _same(pos, device, name)
-    return pos.to(torch.int32).contiguous()
+    if pos.dtype == torch.int64:  # (cut to 32 bits, a position past them could name a row of the table)
+        pos = pos.clamp(-1, 0x7FFFFFFF).to(torch.int32)
+    return pos.contiguous()
 
 
 def _ptr(x):
@@ -185,7 +187,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight=None, k_weight=None,
     """(q_out, k_out): head norms and rotation of q [..., S, H_q, D] and k [..., S_k, H_k, D].
 
     ``q_weight`` / ``k_weight`` [D] (dtype T or float32) switch the norms on;
-    ``table`` is ``rotary_table``'s.  ``q_positions`` [..., S] (integers) default
+    ``table`` is ``rotary_table``'s.  ``q_positions`` [..., S] (int32 or int64) default
     to 0 .. S-1 along S; ``k_positions`` to q's where the two shapes agree, else
     to 0 .. S_k-1.  A position the table does not hold is clamped to its ends and
     raises bit 1 of ``device_status``.  Inputs may be strided along S (slices of
