@@ -134,6 +134,10 @@ ATTEND = [
     (torch.float32, [(40, 200), (7, 64)], 8, 4, 40, 96, 16, False),
     (torch.float32, [(130, 300), (1, 77)], 4, 1, 128, 64, 64, True),
     (torch.float32, [(257, 300)], 2, 2, 64, 64, 16, True),
+    (torch.float32, [(5, 333), (1, 90), (2, 7)], 3, 1, 8, 24, 256, False),                              # tiles of 8 rows, part filled
+    (torch.float32, [(3, 500), (1, 41), (0, 70)], 10, 2, 96, 72, 16, True),
+    (torch.float32, [(1, 3000), (14, 60), (1, 2), (2, 1)], 1, 1, 64, 128, 64, True),
+    (torch.float32, [(1, 40), (1, 0), (1, 1200)], 16, 1, 128, 64, 16, True),
 ]
 
 

@@ -21,10 +21,13 @@ int bucket_of(int64_t D, int64_t D_v) { return std::max(D, D_v) <= 64 ? 64 : 128
 // ragged to 8192 keys x 8 heads 57 and 90; 64 x 1000 keys, 8 / 16 / 32 rows, 58 / 63
 // / 84 and 75 / 77 / 79; one token of 32 heads to a KV head, 8 x 4096 keys, 62 and
 // 18), while a chunk in the few-row kernel reads its keys once every 16 rows.
-// fp32: the few-row kernel, its row tiles from the mean of packed rows.
+// fp32: the few-row kernel, its row tiles from the mean of packed rows: a thin
+// tile of 8 a warp up to two of them (16 x 8192 keys x 2 heads x 128, 16 rows: 103 us
+// against 135 with tiles of 16 in pairs; 16 x 2000 keys x 4 heads, 12 rows: 61 and 78),
+// then two and four tiles of 16 that share a ring.
 struct Plan {
   bool tc;
-  int mt;  // row tiles of 16 of a group of warps
+  int mt;  // row tiles of a group of warps
 };
 Plan plan_of(int dtype, int64_t tokens, int64_t seqs, int64_t group) {
   if (dtype == SDPA_B200_F16 && group <= 128) return {group > 16 || (tokens > seqs && (tokens - seqs + 1) * group > 16), 1};

@@ -123,20 +123,29 @@ __device__ __forceinline__ int key_tiles(const SeqLens& s) { return s.held > 0 ?
 
 // Shapes of one instantiation.  DB: feature bucket; MT: row tiles (warps) of a
 // group, which shares one ring.
+//
+// fp32 with one row tile is thin: 8 rows.  Q's low parts take rows 8-15 of the
+// first product, so q_hi k + q_lo k is one instruction and Q K^T takes two
+// a step, not three; the second product is O^T = V^T P^T, 16 features x 8 rows,
+// whose P^T operand is the scores' own layout.  Half the sums' registers and no
+// part of Q in shared memory let three CTAs of D = 128 on an SM, not two (32 x 8192 keys x
+// 8 heads x 128, 4 rows: 329 us, 6.5 TB/s; 371 with two, 493 with 16 rows).
 template <typename T, int DB, int MT>
 struct Shape {
   static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr bool kThin = !kHalf && MT == 1;
   static constexpr int kKeys = kHalf ? 16 : 8;              // keys of a block
   static constexpr int kBoxes = DB * static_cast<int>(sizeof(T)) / 128;  // 128-byte column boxes of K, and of V
   static constexpr int kBoxBytes = kKeys * 128;
   static constexpr int kStageBytes = 2 * kBoxes * kBoxBytes;  // 8 KB at DB = 128
-  static constexpr int kCtas = DB == 64 ? 3 : 2;            // resident CTAs an SM
+  static constexpr int kCtas = DB == 64 || kThin ? 3 : 2;  // resident CTAs an SM
   static constexpr int kStages = (DB == 64 ? (kHalf ? 4 : 3) : (kHalf ? 3 : 2)) * MT;
   static constexpr int kGroups = kWarps / MT;               // ranges of a CTA
-  static constexpr int kQBytes = kHalf ? 0 : DB / 8 * 512;  // a warp's low parts of Q (fp32)
+  static constexpr int kQBytes = kHalf || kThin ? 0 : DB / 8 * 512;  // a warp's low parts of Q (fp32)
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kSmemBytes = kGroups * kRingBytes + kWarps * kQBytes + 1024;  // + alignment slack
-  static constexpr int kRowsAll = kRows * MT;
+  static constexpr int kTileRows = kThin ? 8 : kRows;
+  static constexpr int kRowsAll = kTileRows * MT;
 };
 
 // One output row's four columns from its sums (and, where asked, its stats):
@@ -173,11 +182,11 @@ template <typename T, int DB, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
   using S = Shape<T, DB, MT>;
-  constexpr bool HALF = S::kHalf;
+  constexpr bool HALF = S::kHalf, THIN = S::kThin;
   constexpr int KEYS = S::kKeys, ST = S::kStages, BX = S::kBoxes;
   constexpr int KN = KEYS / 8;                 // score column tiles of a block
   constexpr int KS = HALF ? DB / 16 : DB / 8;  // inner steps of Q K^T
-  constexpr int NO = DB / 8;                   // output column tiles
+  constexpr int NO = THIN ? DB / 16 : DB / 8;  // output tiles
   constexpr int ROWS = S::kRowsAll;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = tc::align1024(smem_raw);
@@ -319,9 +328,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
 
     // ---- rows of this warp
     const int total_rows = sl.count * p.G;
-    const int r0 = (rtile * MT + mt) * kRows;
+    const int r0 = (rtile * MT + mt) * S::kTileRows;
     const int ra = r0 + g, rb = r0 + g + 8;
-    const bool va = ra < total_rows, vb = rb < total_rows;
+    const bool va = ra < total_rows, vb = !THIN && rb < total_rows;
     const int shift = sl.held - sl.count;  // position of the first new token
     // keys a row sees: [0, lim)
     const int lim_a = p.causal ? min(sl.held, shift + ra / p.G + 1) : sl.held;
@@ -345,7 +354,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
         uint32_t lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(qf[i][e]), qf[i][e], lo[e]);
-        q_lo[i * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (THIN)
+          qf[i][1] = lo[0], qf[i][3] = lo[2];
+        else
+          q_lo[i * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
 
@@ -399,14 +411,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
             ldmatrix4(k_at + (k2 >> 2) * S::kBoxBytes + k_off + (((2 * (k2 & 3) + k_chunk) ^ sw) << 4), b[h]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) split_fast(__uint_as_float(b[h][e]), b[h][e], bl[h][e]), part[h][e] = 0.0f;
-            l[2 * h] = q_lo[k2 * 32], l[2 * h + 1] = q_lo[(k2 + 1) * 32];
+            if (!THIN) l[2 * h] = q_lo[k2 * 32], l[2 * h + 1] = q_lo[(k2 + 1) * 32];
           }
           // two sums in turn: a product waits 21 cycles for the last one of its sum, 8 for another's
+          if (!THIN) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              mma_1688(part[h], reinterpret_cast<const uint32_t*>(&l[2 * h + x]), b[h][2 * x], b[h][2 * x + 1]);
+              for (int h = 0; h < 2; ++h)
+                mma_1688(part[h], reinterpret_cast<const uint32_t*>(&l[2 * h + x]), b[h][2 * x], b[h][2 * x + 1]);
+          }
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -418,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[0][e] += part[h][e];
+            for (int e = 0; e < 4; ++e) s[0][THIN ? e & 1 : e] += part[h][e];
         }
       }
       // online softmax in log2 units
@@ -431,22 +445,27 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
           const int key = key0 + 8 * a + 2 * t;
           if (key >= lim_a) s[a][0] = -INFINITY;
           if (key + 1 >= lim_a) s[a][1] = -INFINITY;
-          if (key >= lim_b) s[a][2] = -INFINITY;
-          if (key + 1 >= lim_b) s[a][3] = -INFINITY;
+          if (!THIN && key >= lim_b) s[a][2] = -INFINITY;
+          if (!THIN && key + 1 >= lim_b) s[a][3] = -INFINITY;
         }
         mx_a = fmax3(mx_a, s[a][0], s[a][1]);
-        mx_b = fmax3(mx_b, s[a][2], s[a][3]);
+        if (!THIN) mx_b = fmax3(mx_b, s[a][2], s[a][3]);
       }
       mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
-      mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
+      if (!THIN) mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
       mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
-      mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
+      if (!THIN) mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
       if (__any_sync(0xffffffffu, mx_a > m_a || mx_b > m_b)) {
-        const float fa = mx_a > m_a ? ex2(m_a - mx_a) : 1.0f, fb = mx_b > m_b ? ex2(m_b - mx_b) : 1.0f;
+        float fa = mx_a > m_a ? ex2(m_a - mx_a) : 1.0f, fb = mx_b > m_b ? ex2(m_b - mx_b) : 1.0f;
         l_a *= fa;
         l_b *= fb;
+        if (THIN) {  // the output's rows are 2t and 2t + 1
+          fb = __shfl_sync(0xffffffffu, fa, 8 * t + 4);
+          fa = __shfl_sync(0xffffffffu, fa, 8 * t);
+        }
 #pragma unroll
-        for (int x = 0; x < NO; ++x) o[x][0] *= fa, o[x][1] *= fa, o[x][2] *= fb, o[x][3] *= fb;
+        for (int x = 0; x < NO; ++x)
+          o[x][0] *= fa, o[x][1] *= THIN ? fb : fa, o[x][2] *= THIN ? fa : fb, o[x][3] *= fb;
         m_a = mx_a;
         m_b = mx_b;
       }
@@ -455,9 +474,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
       for (int a = 0; a < KN; ++a) {
         s[a][0] = ex2(s[a][0] - ua);
         s[a][1] = ex2(s[a][1] - ua);
+        l_a += s[a][0] + s[a][1];
+        if (THIN) continue;  // (no rows g + 8)
         s[a][2] = ex2(s[a][2] - ub);
         s[a][3] = ex2(s[a][3] - ub);
-        l_a += s[a][0] + s[a][1];
         l_b += s[a][2] + s[a][3];
       }
       // O += P V
@@ -473,8 +493,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
         }
       } else {  // inner index t <-> key 2t, t + 4 <-> key 2t + 1; word g of a box row: column g of four tiles
         uint32_t ph[4], pl[4];
-        split_fast(s[0][0], ph[0], pl[0]), split_fast(s[0][2], ph[1], pl[1]);
-        split_fast(s[0][1], ph[2], pl[2]), split_fast(s[0][3], ph[3], pl[3]);
+        split_fast(s[0][0], ph[0], pl[0]), split_fast(s[0][1], ph[2], pl[2]);
+        if (!THIN) split_fast(s[0][2], ph[1], pl[1]), split_fast(s[0][3], ph[3], pl[3]);
 #pragma unroll
         for (int x = 0; x < BX; ++x) {
           const uint8_t* box = at + (BX + x) * S::kBoxBytes;
@@ -483,6 +503,22 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
           split_fast(*reinterpret_cast<const uint4*>(box + (2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4)), h1, l1);
           const uint32_t *xh0 = reinterpret_cast<const uint32_t*>(&h0), *xh1 = reinterpret_cast<const uint32_t*>(&h1);
           const uint32_t *xl0 = reinterpret_cast<const uint32_t*>(&l0), *xl1 = reinterpret_cast<const uint32_t*>(&l1);
+          if (THIN) {  // tile 2x + j: features 32x + 4g + 2j (rows g) and + 1 (rows g + 8)
+            float part[2][4] = {};
+            const uint32_t a[2][4] = {{xh0[0], xh0[1], xh1[0], xh1[1]}, {xh0[2], xh0[3], xh1[2], xh1[3]}};
+            const uint32_t al[2][4] = {{xl0[0], xl0[1], xl1[0], xl1[1]}, {xl0[2], xl0[3], xl1[2], xl1[3]}};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma_1688(part[j], a[j], pl[0], pl[2]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma_1688(part[j], al[j], ph[0], ph[2]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma_1688(part[j], a[j], ph[0], ph[2]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[2 * x + j][e] += part[j][e];
+            continue;
+          }
           float part[4][4] = {};  // (four sums in turn, as above)
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_1688(part[j], pl, xh0[j], xh1[j]);
@@ -536,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     const float inv_a = complete ? row_scale(l_a) : 1.0f, inv_b = complete ? row_scale(l_b) : 1.0f;
     const int64_t oa = static_cast<int64_t>(sl.begin + ra / p.G) * p.H_q + head * p.G + ra % p.G;
     const int64_t ob = static_cast<int64_t>(sl.begin + rb / p.G) * p.H_q + head * p.G + rb % p.G;
-    const int64_t pa = (range * 2 + slot) * ROWS + mt * kRows + g, pb = pa + 8;
+    const int64_t pa = (range * 2 + slot) * ROWS + mt * S::kTileRows + g, pb = pa + 8;
     if (t == 0) {
       if (complete) {
         if (va) p.stats[oa] = row_stats(m_a, l_a);
@@ -558,6 +594,23 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
         } else {
           if (va) *reinterpret_cast<float2*>(p.part_o + pa * DB + col) = make_float2(o[x][0], o[x][1]);
           if (vb) *reinterpret_cast<float2*>(p.part_o + pb * DB + col) = make_float2(o[x][2], o[x][3]);
+        }
+      }
+    } else if (THIN) {  // rows 2t and 2t + 1; features as the product left them
+      const float inv_0 = __shfl_sync(0xffffffffu, inv_a, 8 * t), inv_1 = __shfl_sync(0xffffffffu, inv_a, 8 * t + 4);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = r0 + 2 * t + e;
+        if (row >= total_rows) continue;
+        const float inv = e ? inv_1 : inv_0;
+        float* const dst = complete ? static_cast<float*>(p.out) +
+                                          (static_cast<int64_t>(sl.begin + row / p.G) * p.H_q + head * p.G + row % p.G) * p.D_v
+                                    : p.part_o + (pa - g + 2 * t + e) * DB;
+#pragma unroll
+        for (int x = 0; x < BX; ++x) {
+          const int col = 32 * x + 4 * g;
+          if (!complete || col < p.D_v)
+            store4<float>(dst + col, o[2 * x][e] * inv, o[2 * x][e + 2] * inv, o[2 * x + 1][e] * inv, o[2 * x + 1][e + 2] * inv);
         }
       }
     } else {
