@@ -460,12 +460,11 @@ __device__ __forceinline__ void backward_heads(const Raw<T> (&in)[N][4], T* dx, 
 // A block walks tokens blockIdx.x, + gridDim.x, .. (grid.y: shares of the heads
 // when there are few tokens), summing dw in registers; its sums go to
 // partial[block][q, k][D], added by weight_kernel in block order (no atomics: the
-// same bits every run).  RING: the loads run kStages - 1 head pairs ahead, through
-// shared memory (at its registers two blocks an SM fit, whose own loads are too few
-// in flight: 151 us against 191 for 32768 tokens x 32 heads x 128 fp16).  Worth it
-// where a group walks several tokens; with one the ring only adds a step (4099 tokens
-// x 16 heads x 64 fp32: 22 us against 16).
-template <typename T, int LANES, bool INTER, bool RING>
+// same bits every run).  The loads run kStages - 1 head pairs ahead, through
+// shared memory: at its registers two blocks an SM fit, whose own loads are too few
+// in flight (8192 tokens x 40 heads x 128 fp16: 61 us against 75 without the ring, 4099 x 32 x 64
+// fp32, two head pairs a group: 25 and 27).
+template <typename T, int LANES, bool INTER>
 __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Params p) {
   constexpr int N = 2, ST = kStages<T>;  // x and dy of two heads a stage
   constexpr int kGroups = kThreads / LANES;
@@ -504,33 +503,20 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const Params p) {
       }
       ring.commit();
     };
-    if (RING) {
 #pragma unroll
-      for (int i = 0; i < ST - 1; ++i) load();
-    }
+    for (int i = 0; i < ST - 1; ++i) load();
     for (int64_t t = g.token; t < s.tokens; t += step) {
       float cs[E], sn[E];
       load_turn(p, c, g.lane, s.positions ? s.positions[t] : static_cast<int>(t) % s.period, cs, sn);
       for (int h = blockIdx.y * N; h < s.heads; h += gridDim.y * N) {
         Raw<T> in[N][4];
-        if (RING) {
-          ring.template wait<ST - 2>();
+        ring.template wait<ST - 2>();
 #pragma unroll
-          for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) in[i][k] = ring.read((stage * N + i) * 4 + k);
-          if (++stage == ST) stage = 0;
-          load();  // into the stage that the last pair has left
-        } else {
-          const T* x = static_cast<const T*>(s.x) + t * s.stride + h * p.D;
-          const T* dy = static_cast<const T*>(s.dy) + t * s.dy_stride + h * p.D;
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (c.live && h + i < s.heads) {
-              if (norm) in[i][0].load(x + i * p.D + c.a), in[i][1].load(x + i * p.D + c.b);
-              in[i][2].load(dy + i * p.D + c.a), in[i][3].load(dy + i * p.D + c.b);
-            }
-        }
+          for (int k = 0; k < 4; ++k) in[i][k] = ring.read((stage * N + i) * 4 + k);
+        if (++stage == ST) stage = 0;
+        load();  // into the stage that the last pair has left
         backward_heads<T, LANES, INTER, N>(in, static_cast<T*>(s.y) + t * s.heads * p.D, s.heads, h, p, c, w, norm, cs, sn,
                                            g.mask, dw);
       }
