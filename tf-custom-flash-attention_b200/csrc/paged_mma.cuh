@@ -8,7 +8,7 @@
 // sequence's new tokens are packed into rows r = token * G + g, 16 to a tile,
 // so all of them share one reading.  The products go through warp-level
 // matrix instructions (m16n8k16 fp16; m16n8k8 tf32 three times a product for
-// fp32): 16 rows are a tenth of a tcgen05 tile, and its operands would have to
+// fp32, whose tiles have 8 rows up to 16 packed rows a sequence: see Shape): 16 rows are a tenth of a tcgen05 tile, and its operands would have to
 // pass through shared memory and TMEM, while these take them from registers.
 //
 // Every warp streams alone: TMA boxes of one block of keys (16 fp16, 8 fp32;

@@ -13,8 +13,8 @@
 // pairs 8j..), weights, cosines and sines are multiplied once a token, and the
 // products go in packed pairs (f32x2).  A group walks the heads of one token,
 // four at a time with all their loads ahead of the arithmetic.  32768 tokens x
-// 32 heads x 128 in fp16: forward 99 us (537 MB, 5.4 TB/s), backward 151 us (805 MB,
-// 5.3 TB/s).  Measured worse: the weights and the turn applied apart (120 us forward);
+// 32 heads x 128 in fp16: forward 99 us (537 MB, 5.4 TB/s); backward of 40 heads 183 us
+// (1007 MB, 5.5 TB/s).  Measured worse: the weights and the turn applied apart (120 us forward);
 // sixteen features a lane, with 16-byte loads and fewer instructions but over 110
 // registers (118 us); the forward's loads through a ring as the backward's (99 us).
 // All arithmetic is fp32, rounded to T once, at the store.
