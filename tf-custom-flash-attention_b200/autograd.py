@@ -13,6 +13,25 @@ import torch
 from . import ops, rotary
 
 
+class _FirstOrder(torch.autograd.Function):
+    """compute() as a function of `inputs` that has no derivative."""
+
+    @staticmethod
+    def forward(ctx, compute, *inputs):
+        return compute()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("sdpa_b200 has no second derivatives: a gradient of an operator was differentiated again")
+
+
+def _first_order(compute, *inputs):
+    """compute(), the gradients an operator's kernel gives.  Its results carry no graph; where autograd builds one
+    (create_graph=True) they get a node over all that they depend on, the saved inputs too, which refuses to be
+    differentiated: without it the terms through them would be left out in silence."""
+    return _FirstOrder.apply(compute, *inputs) if torch.is_grad_enabled() else compute()
+
+
 class SdpaFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seed, offset, dropout, scale, causal_mask, differentiable_stats=False):
@@ -87,14 +106,16 @@ class QKNormRopeFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, table, q_positions, k_positions = ctx.saved_tensors
-        grads = rotary.qk_norm_rope_grad(q, k, dq_out, dk_out, q_weight, k_weight, table, q_positions, k_positions,
-                                         *ctx.attrs)
+        grads = _first_order(lambda: rotary.qk_norm_rope_grad(q, k, dq_out, dk_out, q_weight, k_weight, table, q_positions,
+                                                              k_positions, *ctx.attrs),
+                             q, k, dq_out, dk_out, q_weight, k_weight)
         return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, table=None, q_positions=None, k_positions=None, eps: float = 1e-6,
                  interleaved: bool = False):
-    """Differentiable ``rotary.qk_norm_rope``: gradients for q, k and the norm weights.
+    """Differentiable ``rotary.qk_norm_rope``: gradients for q, k and the norm weights, first derivatives only
+    (differentiating them again raises RuntimeError).
 
     A step captured into a CUDA graph needs leaves of which no eager autograd
     graph is alive (torch would join the capture with the stream of the old one
