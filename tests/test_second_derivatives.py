@@ -66,3 +66,47 @@ def test_rope_terms_beside_it_keep_their_second_derivative(rope_on_cpu):
     gu, _ = torch.autograd.grad(loss, (u, w), create_graph=True)
     (second,) = torch.autograd.grad(gu.sum(), u)
     assert torch.allclose(second, 6 * u)
+
+
+def attend(q, k, v, scale):
+    s = q @ k.transpose(-1, -2) * scale
+    return s.softmax(-1) @ v, s.logsumexp(-1)
+
+
+@pytest.fixture
+def sdpa_on_cpu(monkeypatch):
+    def forward(q, k, v, seed, offset, *, scale, dropout, causal_mask):
+        return attend(q, k, v, scale)
+
+    def backward(q, k, v, o, stats, d_o, seed, offset, *, dropout, scale, causal_mask, d_stats=None):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        with torch.enable_grad():
+            o, s = attend(*leaves, scale)
+        return torch.autograd.grad((o, s), leaves, (d_o.detach(), torch.zeros_like(s) if d_stats is None else d_stats.detach()))
+
+    monkeypatch.setattr(fa.ops, "sdpa", forward)
+    monkeypatch.setattr(fa.ops, "sdpa_grad", backward)
+    monkeypatch.setattr(fa.ops, "sdpa_bshd", lambda *a, **kw: forward(*a, **kw))
+    monkeypatch.setattr(fa.ops, "sdpa_grad_bshd", lambda *a, **kw: backward(*a, **kw))
+
+
+def with_stats(h, differentiable):
+    o, s = fa.autograd.sdpa_with_stats(h, 2 * h, h, 0, 0, differentiable_stats=differentiable)
+    return o * s.detach()[..., None] + (s[..., None] if differentiable else 0)
+
+
+ATTENTIONS = [lambda h: fa.autograd.sdpa(h, 2 * h, h, 0, 0), lambda h: fa.autograd.sdpa_bshd(h, h, h, 0, 0),
+              lambda h: with_stats(h, False), lambda h: with_stats(h, True)]
+
+
+@pytest.mark.parametrize("op", range(4))
+@pytest.mark.parametrize("square", [True, False])
+def test_attention_second_derivative_is_refused(sdpa_on_cpu, op, square):
+    w, x = project()
+    out = ATTENTIONS[op]((x[0] @ w).tanh())
+    loss = (out * out).sum() if square else out.sum()
+    (first,) = torch.autograd.grad(loss, w, retain_graph=True)
+    (g,) = torch.autograd.grad(loss, w, create_graph=True)
+    assert torch.equal(first, g)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad((g * g).sum(), w)

@@ -5,6 +5,8 @@ Mirrors ``@tf.RegisterGradient("Sdpa")`` (mha.py:10-21): the backward of
 seed and offset get no gradient, and the gradient reaching ``stats`` is
 ignored (the reference drops it via ``*args``) unless the caller asks for
 it with ``sdpa_with_stats(..., differentiable_stats=True)`` (an extension).
+Gradients are not differentiable again (as the reference registers none for
+``SdpaGrad``): doing so raises RuntimeError.
 """
 from __future__ import annotations
 
@@ -50,8 +52,10 @@ class SdpaFunction(torch.autograd.Function):
         seed, offset, dropout, scale, causal = ctx.attrs
         if d_o is None:
             d_o = torch.zeros_like(o)
-        dq, dk, dv = ops.sdpa_grad(q, k, v, o, s, d_o.contiguous(), seed, offset, dropout=dropout, scale=scale,
-                                   causal_mask=causal, d_stats=d_stats if ctx.stats_grad else None)
+        d_stats = d_stats if ctx.stats_grad else None
+        dq, dk, dv = _first_order(lambda: ops.sdpa_grad(q, k, v, o, s, d_o.contiguous(), seed, offset, dropout=dropout,
+                                                        scale=scale, causal_mask=causal, d_stats=d_stats),
+                                  q, k, v, d_o, d_stats)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -70,8 +74,9 @@ class SdpaBSHDFunction(torch.autograd.Function):
     def backward(ctx, d_o):
         q, k, v, o, s = ctx.saved_tensors
         seed, offset, dropout, scale, causal = ctx.attrs
-        dq, dk, dv = ops.sdpa_grad_bshd(q, k, v, o, s, d_o.contiguous(), seed, offset, dropout=dropout, scale=scale,
-                                        causal_mask=causal)
+        dq, dk, dv = _first_order(lambda: ops.sdpa_grad_bshd(q, k, v, o, s, d_o.contiguous(), seed, offset,
+                                                             dropout=dropout, scale=scale, causal_mask=causal),
+                                  q, k, v, d_o)
         return dq, dk, dv, None, None, None, None, None
 
 
