@@ -113,11 +113,15 @@ class MHA(torch.nn.Module):
         """New tokens q [T, num_heads*Dh], k, v [T, heads of the cache * Dh] of the batch's sequences, one behind the
         other: keys and values go to the cache (normed and rotated like q), the result is [T, num_heads*Dv].  The
         cache may have fewer heads than num_heads (a divisor: groups of query heads share one).  Inference only:
-        no gradients and no dropout."""
+        no gradients and no dropout.  A sequence longer than max_positions is refused as in forward, by the batch's
+        ``longest``; where that is unknown, or a captured step's lengths grow past it, positions are clamped to the
+        rotation's table and raise bit 1 of ``device_status``."""
         if q.dim() != 2 or k.dim() != 2 or v.dim() != 2:
             raise ValueError("forward_paged takes q, k, v of rank 2 ([tokens, features])")
         if q.shape[1] % self.num_heads:
             raise ValueError(f"num_heads {self.num_heads} does not divide the feature size {q.shape[1]}")
+        if self.rotary_dim and batch.longest is not None and batch.longest > self.max_positions:
+            raise ValueError(f"sequences of {batch.longest} tokens with max_positions {self.max_positions}")
         heads = cache.k_pages.shape[2]
         q3 = q.unflatten(1, (self.num_heads, -1))
         k3, v3 = k.unflatten(1, (heads, -1)), v.unflatten(1, (heads, -1))

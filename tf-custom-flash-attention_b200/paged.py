@@ -188,12 +188,16 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
 
 
 class PagedBatch:
-    """The index tensors of one serving step (``PagedCache.batch``): page_table, kv_len, q_start, and its tokens."""
+    """The index tensors of one serving step (``PagedCache.batch``): page_table, kv_len, q_start, and its tokens.
 
-    __slots__ = ("page_table", "kv_len", "q_start", "tokens")
+    ``longest``: the largest kv_len of a sequence with new tokens, for checks on the host; None where only the device
+    knows the lengths."""
 
-    def __init__(self, page_table, kv_len, q_start, tokens: int):
+    __slots__ = ("page_table", "kv_len", "q_start", "tokens", "longest")
+
+    def __init__(self, page_table, kv_len, q_start, tokens: int, longest: int | None = None):
         self.page_table, self.kv_len, self.q_start, self.tokens = page_table, kv_len, q_start, tokens
+        self.longest = longest
 
 
 class PagedCache:
@@ -245,7 +249,8 @@ class PagedCache:
         index = index.to(self.k_pages.device)  # one copy for the three
         n = len(rows)
         table, kv_len, q_start = index.split([n * width, n, n + 1])
-        return PagedBatch(table.view(n, width), kv_len, q_start, start[-1])
+        return PagedBatch(table.view(n, width), kv_len, q_start, start[-1],
+                          max((self._length[s] for s, c in new_tokens if c), default=0))
 
     def free(self, sequence):
         self._free.extend(reversed(self._pages.pop(sequence, [])))
