@@ -44,3 +44,18 @@ def test_paged_layer_takes_the_last_position_of_its_table():
     with pytest.raises(ValueError, match="max_positions"):
         m.forward_paged(x[:1], x[:1], x[:1], c, batch)
     assert torch.equal(before, c.k_pages) and fa.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [dict(max_positions=64), dict(rotary_base=100.0), dict(rotary_dim=16)])
+def test_the_rotation_follows_changed_attributes(change):
+    kw = dict(num_heads=2, rotary_dim=32, max_positions=16)
+    m = fa.MHA(**kw).cuda().eval()
+    x = torch.randn(1, 16, 64, device="cuda").half()
+    m(x, x, x)  # (lays its table out)
+    for name, value in change.items():
+        setattr(m, name, value)
+    new = fa.MHA(**{**kw, **change}).cuda().eval()
+    y = torch.randn(1, new.max_positions, 64, device="cuda").half()
+    assert torch.equal(m(y, y, y), new(y, y, y))
+    assert fa.device_status() == 0

@@ -46,19 +46,20 @@ class MHA(torch.nn.Module):
         if qk_norm_dim is not None:
             self.q_norm = torch.nn.Parameter(torch.ones(qk_norm_dim))
             self.k_norm = torch.nn.Parameter(torch.ones(qk_norm_dim))
-        self._rotary_tables: dict = {}  # by device: made from the arguments alone
+        self._rotary_tables: dict = {}  # by device and the three arguments (kept: a captured graph may read an older one)
 
     def _table(self, device):
-        """The rotation's table on `device`, laid out once."""
+        """The rotation's table on `device`, laid out once for the layer's present arguments."""
         if not self.rotary_dim:
             return None
-        if device not in self._rotary_tables:
+        key = device, self.max_positions, self.rotary_dim, self.rotary_base
+        if key not in self._rotary_tables:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call the layer once before capturing it: its rotation table is not laid out yet")
             table = rotary.rotary_table(self.max_positions, self.rotary_dim, self.rotary_base, device)
             torch.cuda.current_stream(device).synchronize()  # later calls may come from any stream
-            self._rotary_tables[device] = table
-        return self._rotary_tables[device]
+            self._rotary_tables[key] = table
+        return self._rotary_tables[key]
 
     def _norm_rope(self, q4: torch.Tensor, k4: torch.Tensor):
         """Norms and rotation of q4, k4 [B, S, H, Dh] at positions 0 .. S-1 (nothing without either)."""
