@@ -85,14 +85,15 @@ __device__ __forceinline__ void mma_1688(float* d, const uint32_t* a, uint32_t b
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, both tf32 values, by Veltkamp's splitting: hi is x rounded to 11
-// bits, lo the rest (exact) cut to 11.  (The conversion instruction runs at a
-// fraction of the rate; adding half a step to the bits loses the NaN of all ones.)
+// x = hi + lo, both tf32 values: hi is x rounded to 11 bits, by half a step added
+// to its bits (a carry moves on into the exponent), lo the rest (exact) cut to
+// 11.  Finite for |x| < 2^128 (1 - 2^-12).  A NaN stays one in lo, which every
+// product takes part of, whatever its bits become in hi; an infinity gives NaN.
+// (The conversion instruction runs at a fraction of the rate; splitting by the
+// product with 2^13 + 1 takes one instruction more and overflows from 2^115 on.)
 __device__ __forceinline__ void split_fast(float x, uint32_t& hi, uint32_t& lo) {
-  const float c = __fmul_rn(x, 8193.0f);  // (each step rounded by itself, not fused)
-  const float h = __fsub_rn(c, __fsub_rn(c, x));
-  hi = __float_as_uint(h);
-  lo = __float_as_uint(__fsub_rn(x, h)) & 0xffffe000u;
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi))) & 0xffffe000u;
 }
 __device__ __forceinline__ void split_fast(const uint4& x, uint4& hi, uint4& lo) {
   split_fast(__uint_as_float(x.x), hi.x, lo.x);

@@ -139,7 +139,10 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     (output, stats) to write into, memory apart from q's; rows behind the last sequence keep what they
     held (and hold anything in a result allocated here).  A NaN or infinity
     cached behind a sequence's kv_len reaches nothing; one at a position that
-    only later tokens of the same chunk see may reach the chunk's earlier rows."""
+    only later tokens of the same chunk see may reach the chunk's earlier rows.
+    In float, products are taken of two parts of each value: an infinity gives
+    NaN, finite values may have any size up to 2^128 (1 - 2^-12) as long as
+    scores and sum_j exp(score_j - max) v_j stay in float's range."""
     dt = _dtype_of(q)
     if q.dim() != 3:
         raise InvalidArgumentError(f"q must be [T, H_q, D] but is rank {q.dim()}")
