@@ -7,7 +7,11 @@
 // device and are read by the kernels, never by the host, so a captured graph
 // follows them.  Entries outside their ranges never reach memory: a page id
 // outside the pool reads as zeros and is not written, lengths are clamped to
-// the table's capacity, and either raises kStatusBadIndex.
+// the table's capacity, starts to the call's tokens, and each raises
+// kStatusBadIndex.  So does a q_start that descends: its sequences would share
+// tokens, and the work that the host launched for (tokens, seqs) would not cover
+// theirs.  The attention then does nothing at all; the cache write, which
+// goes by token, leaves out those that the search finds no sequence for.
 #pragma once
 #include <cstdint>
 
@@ -30,16 +34,19 @@ struct PagedView {
 // so that no index built from them leaves its array.
 struct SeqLens {
   int begin, count, held;
+  bool ascends;  // q_start[n] <= q_start[n + 1]
 };
 __device__ __forceinline__ SeqLens seq_lens(const PagedView& v, int n) {
-  const int a = max(0, min(v.q_start[n], v.tokens)), e = max(a, min(v.q_start[n + 1], v.tokens));
+  const int q0 = v.q_start[n], q1 = v.q_start[n + 1];
+  const int a = max(0, min(q0, v.tokens)), e = max(0, min(q1, v.tokens));
   const long long cap = static_cast<long long>(v.width) << v.page_shift;
   const int held = v.kv_len[n];
   SeqLens s;
   s.begin = a;
-  s.count = e - a;
+  s.ascends = a <= e;
+  s.count = s.ascends ? e - a : 0;
   s.held = held < 0 ? 0 : (held > cap ? static_cast<int>(cap) : held);
-  if (s.held != held) atomicOr(&g_status_word, kStatusBadIndex);
+  if (s.held != held || a != q0 || e != q1 || !s.ascends) atomicOr(&g_status_word, kStatusBadIndex);
   return s;
 }
 
@@ -50,6 +57,17 @@ __device__ __forceinline__ int page_of(const PagedView& v, int n, int i) {
   if (static_cast<unsigned>(p) < static_cast<unsigned>(v.num_pages)) return p;
   atomicOr(&g_status_word, kStatusBadIndex);
   return -1;
+}
+
+// Raises the status for starts that descend or lie outside the call's tokens (the
+// first `threads` of one block; where the work goes by token, not by sequence).
+__device__ __forceinline__ void starts_check(const PagedView& v, int threads) {
+  bool bad = false;
+  for (int n = threadIdx.x; n <= v.seqs; n += threads) {
+    const int a = __ldg(v.q_start + n);
+    bad |= a < 0 || a > v.tokens || (n < v.seqs && __ldg(v.q_start + n + 1) < a);
+  }
+  if (bad) atomicOr(&g_status_word, kStatusBadIndex);
 }
 
 // The sequence that owns token t, or -1 (before the first or behind the last).

@@ -221,8 +221,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
   // ---- this group's range of tiles
   const int per = (p.view.seqs + kThreads - 1) / kThreads;
   int64_t mine = 0;
+  bool descends = false;
   for (int n = tid * per; n < min(p.view.seqs, (tid + 1) * per); ++n) {
     const SeqLens s = seq_lens(p.view, n);
+    descends |= !s.ascends;
     mine += static_cast<int64_t>(row_tiles(p, s, ROWS)) * key_tiles(s);
   }
   mine *= p.H_kv;
@@ -233,13 +235,14 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     if (lane >= d) incl += up;
   }
   if (lane == 31) s_warp[warp] = incl;
-  __syncthreads();
+  const bool refused = __syncthreads_or(descends);
   int64_t before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
+  if (refused) total = 0;  // (see paged.cuh)
   s_before[tid] = before + incl - mine;
   __syncthreads();
   const int64_t range = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(gridDim.x) * group;

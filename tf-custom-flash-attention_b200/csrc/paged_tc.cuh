@@ -201,16 +201,25 @@ __device__ __forceinline__ float warp_max(float x) {
 // The piece that CTA `idx` computes; false if there is none.  Every warp works
 // it out for itself (no barrier, and the same everywhere): lane i takes the
 // i-th share of the sequences.  slots: workspace slots of the call.  (Items and
-// pieces are counted in 32 bits; the host refuses more.)
+// pieces are counted in 32 bits and launched as CTAs; the host bounds both by the
+// call's tokens and sequences, which holds for ascending starts alone: with
+// others there are no pieces and no slots, see paged.cuh.)
 __device__ __forceinline__ bool find_piece(const Params& p, int idx, Piece& out, int& slots) {
   const int lane = threadIdx.x & 31;
   const int tokens2 = 2 * (kBM / p.G);
   const int per = (p.view.seqs + 31) / 32, n0 = lane * per, n1 = min(p.view.seqs, n0 + per);
-  const SeqLens none = {0, 0, 0};
+  const SeqLens none = {0, 0, 0, true};
   const SeqLens s0 = n0 < n1 ? seq_lens(p.view, n0) : none;  // (the only one, up to 32 sequences)
   auto lens = [&](int n) { return n == n0 ? s0 : seq_lens(p.view, n); };
   int items = 0;
-  for (int n = n0; n < n1; ++n) items += pairs_of(lens(n), tokens2);
+  bool descends = false;
+  for (int n = n0; n < n1; ++n) {
+    const SeqLens s = lens(n);
+    items += pairs_of(s, tokens2);
+    descends |= !s.ascends;
+  }
+  slots = 0;
+  if (__any_sync(0xffffffffu, descends)) return false;
   const int items_to = warp_scan(items);
   const int all_items = __shfl_sync(0xffffffffu, items_to, 31) * p.H_kv;
   const bool whole = all_items >= p.sms;  // the first `full` items run whole

@@ -361,10 +361,13 @@ __global__ void __launch_bounds__(kThreads, kAppendBlocks<T>) append_kernel(cons
   };
   int u = blockIdx.y;
   load(u);  // on its way while the token's place is looked up (four dependent reads)
+  if (blockIdx.x == 0 && blockIdx.y == 0) starts_check(p.view, min(static_cast<int64_t>(kThreads), p.view.tokens * int64_t(LANES)));
   const int n = seq_of_token<LANES>(p.view, static_cast<int>(g.token), g.mask, g.lane);
   if (n < 0) return;
   const int64_t held = p.view.kv_len[n];
-  const int64_t pos = held - (p.view.q_start[n + 1] - g.token);
+  const int64_t end = min(p.view.q_start[n + 1], p.view.tokens);
+  if (p.view.q_start[n] > g.token || g.token >= end) return;  // (starts that descend)
+  const int64_t pos = held - (end - g.token);
   const bool in_table = pos >= 0 && pos < (static_cast<int64_t>(p.view.width) << p.view.page_shift);
   const int page = in_table ? page_of(p.view, n, static_cast<int>(pos >> p.view.page_shift)) : -1;
   if (!in_table && g.lane == 0) atomicOr(&g_status_word, kStatusBadIndex);

@@ -12,9 +12,13 @@ so new token i of sequence n is at position kv_len[n] - (q_start[n+1] -
 q_start[n]) + i.  The kernels read these on the device, the host never does: a
 captured graph replays with whatever they hold then.  Rows behind the last
 sequence (T past q_start[N], the padding of a captured batch) are neither
-written to the cache nor to the outputs.  A page id outside the pool reads as
-zeros and is not written, a length past the table's capacity is clamped to it,
-and both raise bit 1 of ``device_status``.
+written to the cache nor to the outputs.  Values outside their ranges reach no
+memory and raise bit 1 of ``device_status``: a page id outside the pool reads
+as zeros and is not written; a length past the table's capacity is clamped to
+it by the attention, and a token whose position is past the table (or below
+zero) is not written; starts are clamped to 0 .. T.  q_start ascends: where it does not,
+the attention leaves the whole call out (its outputs stay as they were), and
+which tokens the write takes is not defined.
 
 ``paged_append`` writes new keys and values, with the head norms and the
 position rotation of ``rotary.qk_norm_rope`` applied on the way (and to the
