@@ -226,7 +226,7 @@ int sdpa_b200_qk_norm_rope_bwd(int dtype, const void* q, const void* dq_out, int
  *
  * append writes k [tokens, H_kv, D] (normed and rotated by its position) and v
  * [tokens, H_kv, D_v] to the pools, and q (NULL: none), normed and rotated
- * likewise, to q_out [tokens, H_q, D]. */
+ * likewise, to q_out [tokens, H_q, D].  Inputs must not overlap what is written. */
 int sdpa_b200_paged_append(int dtype, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                            int64_t v_stride, int64_t tokens, int64_t H_q, int64_t H_kv, int64_t D, int64_t D_v,
                            const void* q_weight, const void* k_weight, int weight_dtype, float eps, const float* table,
@@ -238,8 +238,9 @@ int sdpa_b200_paged_append(int dtype, const void* q, int64_t q_stride, const voi
 /* Attention of new tokens q [tokens, H_q, D] over their sequences' cached keys:
  * out [tokens, H_q, D_v], stats [tokens, H_q] as in sdpa_b200_fwd.  H_q is a
  * multiple of H_kv (query head h reads KV head h / (H_q / H_kv)).  causal != 0:
- * a token sees the keys up to its own position; else all kv_len.  The workspace
- * (16-byte aligned) is the caller's until the call's work has finished. */
+ * a token sees the keys up to its own position; else all kv_len.  Outputs must
+ * not overlap inputs.  The workspace (16-byte aligned) is the caller's until the
+ * call's work has finished. */
 size_t sdpa_b200_paged_workspace_bytes(int dtype, int64_t tokens, int64_t seqs, int64_t H_q, int64_t H_kv, int64_t D,
                                        int64_t D_v);
 int sdpa_b200_paged_sdpa(int dtype, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* out,

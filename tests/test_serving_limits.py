@@ -59,3 +59,25 @@ def test_the_rotation_follows_changed_attributes(change):
     y = torch.randn(1, new.max_positions, 64, device="cuda").half()
     assert torch.equal(m(y, y, y), new(y, y, y))
     assert fa.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_results_may_not_lie_over_any_input_or_each_other():
+    mem = torch.zeros(1 << 16, device="cuda", dtype=torch.float16)
+    q, k_pages, v_pages = mem[:512].view(2, 4, 64), mem[4096:4096 + 4096].view(2, 16, 2, 64), mem[8192:8192 + 4096].view(2, 16, 2, 64)
+    i32 = mem[16384:16384 + 64].view(torch.int32)
+    i32.copy_(torch.tensor([0, 1, 2] + [0, 1] + [5, 9] + [0] * 25, dtype=torch.int32))
+    q_start, page_table, kv_len = i32[:3], i32[3:5].view(2, 1), i32[5:7]
+    args = (q, k_pages, v_pages, page_table, kv_len, q_start)
+    out, stats = torch.empty(2, 4, 64, device="cuda", dtype=torch.float16), torch.empty(2, 4, device="cuda")
+    lie = lambda at, n: mem[at:at + n]
+    for at, name in ((0, "q"), (8184, "k_pages"), (8192 + 4088, "v_pages"), (16384, "q_start|kv_len|page_table")):
+        with pytest.raises(fa.InvalidArgumentError, match=rf"out\[0\] must not share memory with ({name})"):
+            fa.paged_sdpa(*args, out=(lie(at, 512).view(2, 4, 64), stats))
+        with pytest.raises(fa.InvalidArgumentError, match=rf"out\[1\] must not share memory with ({name})"):
+            fa.paged_sdpa(*args, out=(out, lie(at, 16).view(torch.float32).view(2, 4)))
+    with pytest.raises(fa.InvalidArgumentError, match="out.0. and out.1."):
+        fa.paged_sdpa(*args, out=(lie(20000, 512).view(2, 4, 64), lie(20504, 16).view(torch.float32).view(2, 4)))
+    got = fa.paged_sdpa(*args, out=(lie(512, 512).view(2, 4, 64), lie(1024, 16).view(torch.float32).view(2, 4)))  # between them
+    want = fa.paged_sdpa(*args)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and fa.device_status() == 0

@@ -87,7 +87,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     rotated by their position, before they are written; ``q`` [T, H_q, D] gets
     the same (with ``q_weight``) and is returned, else None.  Rows of the result
     behind the last sequence are not written.  Positions that two sequences
-    share (a page entered in both tables) must get the same rows from both."""
+    share (a page entered in both tables) must get the same rows from both, and
+    k, v and q may lie in the pools only in rows that the call does not write."""
     dt = _dtype_of(k)
     if k.dim() != 3:
         raise InvalidArgumentError(f"k must be [T, H_kv, D] but is rank {k.dim()}")
@@ -120,12 +121,21 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     return q_out
 
 
+def _span(x: torch.Tensor):
+    """First byte and end of the stretch of memory that holds a tensor's elements (strides are not negative)."""
+    at = x.data_ptr()
+    if x.is_contiguous():
+        return at, at + x.nbytes
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+
+
+def _meet(a, b) -> bool:
+    return a[0] < b[1] and b[0] < a[1] and a[0] < a[1] and b[0] < b[1]
+
+
 def _share_bytes(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the stretches of memory from the first to the last element of two tensors meet (strides are not negative)."""
-    if not a.numel() or not b.numel():
-        return False
-    end = [x.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size() for x in (a, b)]
-    return a.data_ptr() < end[1] and b.data_ptr() < end[0]
+    """Whether the stretches of memory of two tensors meet."""
+    return _meet(_span(a), _span(b))
 
 
 _workspace_bytes: dict = {}  # of paged_sdpa, by what the query depends on
@@ -140,7 +150,7 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     H_kv; query head h reads KV head h // (H_q / H_kv).  With ``causal_mask`` a
     token sees the keys up to its own position, else all kv_len of its sequence;
     one that sees none gets zeros and stats of -1e9.  ``out`` may pass
-    (output, stats) to write into, memory apart from q's; rows behind the last sequence keep what they
+    (output, stats) to write into, memory apart from the inputs'; rows behind the last sequence keep what they
     held (and hold anything in a result allocated here).  A NaN or infinity
     cached behind a sequence's kv_len reaches nothing; one at a position that
     only later tokens of the same chunk see may reach the chunk's earlier rows.
@@ -172,9 +182,16 @@ def paged_sdpa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
             raise InvalidArgumentError("out[1] must be a contiguous float32 [T, H_q] tensor")
         _same(o, device, "out[0]")
         _same(stats, device, "out[1]")
-        for x, name in ((o, "out[0]"), (stats, "out[1]")):
-            if _share_bytes(x, q):
-                raise InvalidArgumentError(f"{name} must not share memory with q, whose rows other blocks still read")
+        # (other blocks still read what one has written over)
+        at = (("q", _span(q)), ("k_pages", _span(k_pages)), ("v_pages", _span(v_pages)), ("page_table", _span(page_table)),
+              ("kv_len", _span(kv_len)), ("q_start", _span(q_start)))
+        to = _span(o), _span(stats)
+        for i in (0, 1):
+            for name, span in at:
+                if _meet(to[i], span):
+                    raise InvalidArgumentError(f"out[{i}] must not share memory with {name}")
+        if _meet(*to):
+            raise InvalidArgumentError("out[0] and out[1] must not share memory")
     if T == 0 or N == 0:
         return o, stats
     qx, qs = _rows(q, H_q * D, 8 if dt == _lib.F16 else 4)
