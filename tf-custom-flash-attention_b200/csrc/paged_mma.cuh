@@ -8,8 +8,10 @@
 // sequence's new tokens are packed into rows r = token * G + g, 16 to a tile,
 // so all of them share one reading.  The products go through warp-level
 // matrix instructions (m16n8k16 fp16; m16n8k8 tf32 three times a product for
-// fp32, whose tiles have 8 rows up to 16 packed rows a sequence: see Shape): 16 rows are a tenth of a tcgen05 tile, and its operands would have to
-// pass through shared memory and TMEM, while these take them from registers.
+// fp32, the product of the two low parts, 2^-22 of it, left out; its tiles have 8
+// rows up to 16 packed rows a sequence: see Shape): 16 rows are a tenth of a tcgen05
+// tile, and its operands would have to pass through shared memory and TMEM, while
+// these take them from registers.
 //
 // Every warp streams alone: TMA boxes of one block of keys (16 fp16, 8 fp32;
 // always inside one page) go to the warp's own ring of kStages blocks in shared
@@ -130,7 +132,7 @@ __device__ __forceinline__ int key_tiles(const SeqLens& s) { return s.held > 0 ?
 // a step, not three; the second product is O^T = V^T P^T, 16 features x 8 rows,
 // whose P^T operand is the scores' own layout.  Half the sums' registers and no
 // part of Q in shared memory let three CTAs of D = 128 on an SM, not two (32 x 8192 keys x
-// 8 heads x 128, 4 rows: 329 us, 6.5 TB/s; 371 with two, 493 with 16 rows).
+// 8 heads x 128, 4 rows: 336 us, 6.4 TB/s; about 40 us more with two, 160 with 16 rows).
 template <typename T, int DB, int MT>
 struct Shape {
   static constexpr bool kHalf = sizeof(T) == 2;
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
         l_b += s[a][2] + s[a][3];
       }
       // O += P V
-      if (HALF) {  // p in [0, 1] enters the product as fp16 (relative error 2^-12 at most; the sum l keeps fp32)
+      if (HALF) {  // p in [0, 1] enters the product as fp16 (relative error 2^-11 at most; the sum l keeps fp32)
         const uint32_t pa[4] = {pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]),
                                 pack_half2(s[KN - 1][0], s[KN - 1][1]), pack_half2(s[KN - 1][2], s[KN - 1][3])};
 #pragma unroll

@@ -264,8 +264,9 @@ constexpr int kStages = sizeof(T) == 2 ? 4 : 2;
 template <typename T>
 constexpr int kStageBytes = 8 * kThreads * E * static_cast<int>(sizeof(T));
 // Blocks an SM (fp32 holds twice the loads): forward (fp16: 64 registers a
-// thread), and append, whose addresses would spill there (5251 tokens x 48 heads
-// x 128 fp16: 35 us against 37 with four blocks, 46 with two).
+// thread, 44 bytes of them spilled), and append, whose addresses take more (fp16:
+// 80 registers and 64 bytes spilled; 5251 tokens x 48 heads x 128: 35 us against 37
+// with four blocks, 46 with two).
 template <typename T>
 constexpr int kBlocks = sizeof(T) == 2 ? 4 : 3;
 template <typename T>
