@@ -28,6 +28,11 @@ def test_paged_layer_refuses_positions_past_its_table():
     with pytest.raises(ValueError, match="21 tokens with max_positions 20"):
         m.forward_paged(x, x, x, c, batch)
     assert not c.k_pages.any() and not c.v_pages.any()
+    import types
+    m._table = lambda device: None
+    bare = types.SimpleNamespace(page_table=batch.page_table, kv_len=batch.kv_len, q_start=batch.q_start)
+    with pytest.raises(fa.InvalidArgumentError, match="CUDA tensors only"):  # (as far as the write, where nothing is known)
+        m.forward_paged(x, x, x, c, bare)
     plain = fa.MHA(num_heads=2).eval()  # without a rotation there is no table to leave
     with pytest.raises(fa.InvalidArgumentError, match="CUDA tensors only"):
         plain.forward_paged(x, x, x, c, batch)

@@ -121,8 +121,9 @@ class MHA(torch.nn.Module):
             raise ValueError("forward_paged takes q, k, v of rank 2 ([tokens, features])")
         if q.shape[1] % self.num_heads:
             raise ValueError(f"num_heads {self.num_heads} does not divide the feature size {q.shape[1]}")
-        if self.rotary_dim and batch.longest is not None and batch.longest > self.max_positions:
-            raise ValueError(f"sequences of {batch.longest} tokens with max_positions {self.max_positions}")
+        longest = getattr(batch, "longest", None)  # (any object with the index tensors will do)
+        if self.rotary_dim and longest is not None and longest > self.max_positions:
+            raise ValueError(f"sequences of {longest} tokens with max_positions {self.max_positions}")
         heads = cache.k_pages.shape[2]
         q3 = q.unflatten(1, (self.num_heads, -1))
         k3, v3 = k.unflatten(1, (heads, -1)), v.unflatten(1, (heads, -1))
