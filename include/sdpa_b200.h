@@ -221,8 +221,9 @@ int sdpa_b200_qk_norm_rope_bwd(int dtype, const void* q, const void* dq_out, int
  * page page_table[n][j / page_size] (table_width entries a sequence; entries
  * past a sequence's keys are not read).  Tokens behind the last sequence are
  * left alone, in the pools and in the outputs.  Starts outside 0 .. tokens are
- * clamped; a q_start that descends leaves the attention's call out, and which
- * tokens append writes is then not defined (both raise the status bit).
+ * clamped.  Where q_start descends, the sequence between is empty; the attention
+ * leaves the call out if others then share tokens, and which tokens append writes
+ * is not defined.  (All raise the status bit.)
  *
  * append writes k [tokens, H_kv, D] (normed and rotated by its position) and v
  * [tokens, H_kv, D_v] to the pools, and q (NULL: none), normed and rotated

@@ -39,7 +39,7 @@ DESCENDING = [
 
 @pytest.mark.parametrize("case", DESCENDING)
 @pytest.mark.parametrize("causal", [True, False])
-def test_descending_starts_leave_the_call_out(case, causal):
+def test_shared_tokens_leave_the_call_out(case, causal):
     dtype, T, starts, held, hq, hkv = case
     s = step(*case)
     fa.device_status()
@@ -51,6 +51,20 @@ def test_descending_starts_leave_the_call_out(case, causal):
     good = step(dtype, T, [0, T], max(T, held), hq, hkv)
     base.check_attend(good, lens, 0.125, causal, fa.paged_sdpa(**good, scale=0.125, causal_mask=causal))
     assert fa.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,T,hq", [(H16, 5, 2), (H16, 300, 4), (H16, 200, 130), (F32, 5, 1), (F32, 90, 4)])
+@pytest.mark.parametrize("empty", [0, 40, 200])
+def test_descending_starts_that_share_nothing(dtype, T, hq, empty):
+    """Unused places of a batch left at zero: empty to the attention, whose rows are those of the used ones; reported."""
+    lens = [(2, 40), (T - 2, T + 30)] + [(0, 50)] * (empty + 1)
+    s = base.make(dtype, lens, hq, 2 if hq == 4 else 1, 64, 64, 16, seed=3)
+    want = fa.paged_sdpa(**s, scale=0.125)
+    assert fa.device_status() == 0
+    s["q_start"][3:] = 0
+    got = fa.paged_sdpa(**s, scale=0.125)
+    assert fa.device_status() == 2
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 @pytest.mark.parametrize("case", DESCENDING)

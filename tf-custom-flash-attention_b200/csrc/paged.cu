@@ -19,11 +19,12 @@ int bucket_of(int64_t D, int64_t D_v) { return std::max(D, D_v) <= 64 ? 64 : 128
 // groups of up to 128 heads, what its row tiles hold.  (The bound knows no single
 // sequence's tokens: drafts of a few tokens each in many sequences go to the
 // tcgen05 kernel though their rows are few, and a chunk among as many sequences
-// without new tokens to the few-row one, where it is right but slow.)  It serves single tokens among chunks as well
-// (few-row and tcgen05 kernel, us: 16 x 32768 keys x 4 heads 181 and 178; 32
-// ragged to 8192 keys x 8 heads 57 and 90; 64 x 1000 keys, 8 / 16 / 32 rows, 58 / 63
-// / 84 and 75 / 77 / 79; one token of 32 heads to a KV head, 8 x 4096 keys, 62 and
-// 18), while a chunk in the few-row kernel reads its keys once every 16 rows.
+// without new tokens to the few-row one, where it is right but slow.)  It serves
+// single tokens among chunks as well (few-row and tcgen05 kernel, us: 16 x 32768
+// keys x 4 heads 181 and 178; 32 ragged to 8192 keys x 8 heads 57 and 90; 64 x 1000
+// keys, 8 / 16 / 32 rows, 58 / 63 / 84 and 75 / 77 / 79; one token of 32 heads to a
+// KV head, 8 x 4096 keys, 62 and 18), while a chunk in the few-row kernel reads its
+// keys once every 16 rows.
 // fp32: the few-row kernel, its row tiles from the mean of packed rows: a thin
 // tile of 8 a warp up to two of them (16 x 8192 keys x 2 heads x 128, 16 rows: 99 us
 // against 127 with tiles of 16 in pairs; 16 x 2000 keys x 4 heads, 12 rows: 57 and 73),

@@ -8,10 +8,11 @@
 // follows them.  Entries outside their ranges never reach memory: a page id
 // outside the pool reads as zeros and is not written, lengths are clamped to
 // the table's capacity, starts to the call's tokens, and each raises
-// kStatusBadIndex.  So does a q_start that descends: its sequences would share
-// tokens, and the work that the host launched for (tokens, seqs) would not cover
-// theirs.  The attention then does nothing at all; the cache write, which
-// goes by token, leaves out those that the search finds no sequence for.
+// kStatusBadIndex.  So does a q_start that descends: a sequence between two
+// descending starts is empty, and where others then share tokens (the work that
+// the host launched for (tokens, seqs) would not cover theirs) the attention
+// does nothing at all.  The cache write, which goes by token, leaves out those
+// that its search finds no sequence for.
 #pragma once
 #include <cstdint>
 
@@ -48,6 +49,19 @@ __device__ __forceinline__ SeqLens seq_lens(const PagedView& v, int n) {
   s.held = held < 0 ? 0 : (held > cap ? static_cast<int>(cap) : held);
   if (s.held != held || a != q0 || e != q1 || !s.ascends) atomicOr(&g_status_word, kStatusBadIndex);
   return s;
+}
+
+// Whether two sequences share tokens, which takes starts that descend somewhere
+// (callers ask then alone).
+__device__ __forceinline__ bool seqs_overlap(const PagedView& v) {
+  int last = 0;
+  for (int n = 0; n < v.seqs; ++n) {
+    const SeqLens s = seq_lens(v, n);
+    if (s.count == 0) continue;
+    if (s.begin < last) return true;
+    last = s.begin + s.count;
+  }
+  return false;
 }
 
 // Pool page of entry i of sequence n, or -1 (status raised) for an id outside

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DB, MT>::kCtas)
     if (lane >= d) incl += up;
   }
   if (lane == 31) s_warp[warp] = incl;
-  const bool refused = __syncthreads_or(descends);
+  const bool refused = __syncthreads_or(descends) && seqs_overlap(p.view);
   int64_t before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {

@@ -202,8 +202,8 @@ __device__ __forceinline__ float warp_max(float x) {
 // it out for itself (no barrier, and the same everywhere): lane i takes the
 // i-th share of the sequences.  slots: workspace slots of the call.  (Items and
 // pieces are counted in 32 bits and launched as CTAs; the host bounds both by the
-// call's tokens and sequences, which holds for ascending starts alone: with
-// others there are no pieces and no slots, see paged.cuh.)
+// call's tokens and sequences, which holds while no two sequences share tokens:
+// where they do there are no pieces and no slots, see paged.cuh.)
 __device__ __forceinline__ bool find_piece(const Params& p, int idx, Piece& out, int& slots) {
   const int lane = threadIdx.x & 31;
   const int tokens2 = 2 * (kBM / p.G);
@@ -219,7 +219,7 @@ __device__ __forceinline__ bool find_piece(const Params& p, int idx, Piece& out,
     descends |= !s.ascends;
   }
   slots = 0;
-  if (__any_sync(0xffffffffu, descends)) return false;
+  if (__any_sync(0xffffffffu, descends) && seqs_overlap(p.view)) return false;
   const int items_to = warp_scan(items);
   const int all_items = __shfl_sync(0xffffffffu, items_to, 31) * p.H_kv;
   const bool whole = all_items >= p.sms;  // the first `full` items run whole

@@ -16,9 +16,10 @@ written to the cache nor to the outputs.  Values outside their ranges reach no
 memory and raise bit 1 of ``device_status``: a page id outside the pool reads
 as zeros and is not written; a length past the table's capacity is clamped to
 it by the attention, and a token whose position is past the table (or below
-zero) is not written; starts are clamped to 0 .. T.  q_start ascends: where it does not,
-the attention leaves the whole call out (its outputs stay as they were), and
-which tokens the write takes is not defined.
+zero) is not written; starts are clamped to 0 .. T.  q_start ascends: a sequence
+between two descending starts is empty to the attention, which leaves the whole call
+out (its outputs stay as they were) where others then share tokens; which
+tokens the write takes is not defined.
 
 ``paged_append`` writes new keys and values, with the head norms and the
 position rotation of ``rotary.qk_norm_rope`` applied on the way (and to the
